@@ -24,6 +24,16 @@ from .kernels import (  # noqa: F401
     tq_prod_quantize,
     unpack_2bit,
 )
+from .dense import (  # noqa: F401
+    PagedStepPlan,
+    dense_workspace,
+    plan_paged_step,
+    release_pages,
+    rotary_append_dense,
+    rotary_embed,
+    rotary_frequencies,
+    split_k_paged_decode_dense,
+)
 from .cache import (  # noqa: F401
     CompressedBuffer,
     CompressedDynamicCache,

@@ -86,6 +86,17 @@ SIGNATURES = {
     "fq_decode_step_host": (_i, [_p, _p, _p, _i, _p, _i, _p, _i64, _p, _p, _p, _p, _p, _i, _p, _i,
                                  _p, _i, _p, _i, _p, _i, _i, _i, _i, _i, _i64, _f, _i, _p, _p, _sz,
                                  _p, _sz, _p]),
+    "fq_plan_paged_step": (_i, [_p, _p, _i, _p, _i64, _i, _i, _p, _i64, _p, _i64, _p, _p, _p, _p, _p,
+                                _p, _p]),
+    "fq_release_pages": (_i, [_p, _p, _i, _p, _i64, _i, _i, _p, _i64, _p, _p, _p]),
+    "fq_rotary_embed": (_i, [_p, _p, _i, _i64, _i, _i, _i, _i, _p, _p, _i, _p, _i, _f, _i, _p, _p,
+                             _p]),
+    "fq_rotary_append_dense": (_i, [_p, _p, _p, _i, _i64, _i, _i, _i, _i, _p, _p, _i, _p, _i, _f, _p,
+                                    _p, _p, _i, _i64, _p, _i, _p]),
+    "fq_dense_paged_decode_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "fq_dense_paged_decode": (_i, [_p, _i, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p,
+                                   _i64, _i, _p, _i, _i, _i, _i, _i, _i64, _f, _i, _p, _p, _p, _sz,
+                                   _p]),
     "fq_paged_tq4_prefill_workspace_bytes": (_sz, [_i, _i, _i]),
     "fq_paged_tq4_prefill": (_i, [_p, _i, _p, _p, _i64, _p, _p, _p, _i, _p, _i, _p, _i, _i, _i, _i,
                                   _i, _i, _i, _i64, _f, _p, _p, _sz, _p]),

@@ -29,7 +29,7 @@ COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-I", INCLUDE
 
 KERNEL_SOURCES = ["capi.cu", "compress.cu", "decompress.cu", "paged_decode.cu", "prefill.cu",
                   "rotate.cu", "host_step.cu", "cache_update.cu",
-                  "decode_multi.cu", "packing.cu"]
+                  "decode_multi.cu", "packing.cu", "dense_decode.cu", "rotary.cu", "step_plan.cu"]
 
 
 def _sources():

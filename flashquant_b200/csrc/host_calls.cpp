@@ -141,7 +141,7 @@ int native(std::mutex* calls, F call) {
   if (calls) lock = std::unique_lock<std::mutex>(*calls);
   return call();
 }
-enum { kDecode = 0, kAttention = 1 };
+enum { kDecode = 0, kAttention = 1, kDense = 2 };
 
 // Bytes for one call: what a call writes and reads back within itself is not shared with another one.
 Tensor call_bytes(int dev, size_t bytes, bool zero) {
@@ -553,6 +553,249 @@ PyObject* cache_update(PyObject*, Args a, Py_ssize_t n) {
   }));
 }
 
+// ------------------------------------------------------------------------------------
+// around 16-bit pages
+// ------------------------------------------------------------------------------------
+// (tokens, heads, head_dim) with adjacent values of a head
+const Tensor* rows(PyObject* o, int dev) {
+  const Tensor* t = on_device(o, dev);
+  return t && t->dim() == 3 && t->stride(2) == 1 ? t : nullptr;
+}
+// no two rows share memory
+bool own_rows(const Tensor& t) {
+  const int64_t n = t.size(0), h = t.size(1), d = t.size(2), s = t.stride(0), u = t.stride(1);
+  return ((h == 1 || u >= d) && (n == 1 || s >= (h - 1) * u + d)) ||
+         ((n == 1 || s >= d) && (h == 1 || u >= (n - 1) * s + d));
+}
+// None makes a new tensor
+bool out_rows(PyObject* o, const Tensor& like, int dev, Tensor& out) {
+  if (o == Py_None) {
+    out = at::empty(like.sizes(), like.options());
+    return true;
+  }
+  const Tensor* t = rows(o, dev);
+  if (!t || t->scalar_type() != like.scalar_type() || t->sizes() != like.sizes() || !own_rows(*t)) return false;
+  out = *t;
+  return true;
+}
+// (num_blocks, block_size, H_kv, D), the values of a row adjacent; `written`: its rows are its own
+const Tensor* pages(PyObject* o, int dev, at::ScalarType st, bool written) {
+  const Tensor* t = on_device(o, dev);
+  if (!t || t->dim() != 4 || t->scalar_type() != st || t->stride(3) != 1) return nullptr;
+  for (int i = 0; written && i < 3; ++i)
+    if (t->size(i) > 1 && t->stride(i) < t->size(3)) return nullptr;
+  return t;
+}
+const Tensor* ints(PyObject* o, int dev, int64_t n) {
+  const Tensor* t = dense(o, dev);
+  return t && t->dim() == 1 && t->size(0) == n &&
+                 (t->scalar_type() == at::kLong || t->scalar_type() == at::kInt)
+             ? t
+             : nullptr;
+}
+const Tensor* frequencies(PyObject* o, int dev, int64_t head_dim) {
+  const Tensor* t = dense(o, dev, at::kDouble);
+  return t && t->dim() == 1 && 2 * t->size(0) <= head_dim ? t : nullptr;
+}
+bool is_long(const Tensor& t) { return t.scalar_type() == at::kLong; }
+PyObject* pair(const Tensor& a, const Tensor* b) {
+  PyObject* t = PyTuple_New(2);
+  if (!t) return nullptr;
+  PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(a));
+  if (!b) Py_INCREF(Py_None);
+  PyTuple_SET_ITEM(t, 1, b ? THPVariable_Wrap(*b) : Py_None);
+  return t;
+}
+
+// (q, k or None, positions, frequencies, layout, scale, inverse, out or None)
+PyObject* rotary_embed(PyObject*, Args a, Py_ssize_t n) {
+  const int dev = n == 8 ? call_device(a[0]) : -1;
+  if (dev < 0) return none();
+  const Tensor *q = rows(a[0], dev), *k = a[1] == Py_None ? nullptr : rows(a[1], dev);
+  int64_t layout;
+  if (!q || (!k && a[1] != Py_None) || dtype_code(*q) < 0 || !as_int(a[4], layout) || !PyFloat_Check(a[5]) ||
+      !PyBool_Check(a[6]))
+    return none();
+  const int64_t tokens = q->size(0), d = q->size(2);
+  const Tensor *pos = ints(a[2], dev, tokens), *freq = frequencies(a[3], dev, d);
+  if (!pos || !freq || (k && (k->size(0) != tokens || k->size(2) != d || k->scalar_type() != q->scalar_type())))
+    return none();
+  PyObject *oq = Py_None, *ok = Py_None;
+  if (a[7] != Py_None) {
+    if (!PyTuple_Check(a[7]) || PyTuple_GET_SIZE(a[7]) != 2) return none();
+    oq = PyTuple_GET_ITEM(a[7], 0);
+    ok = PyTuple_GET_ITEM(a[7], 1);
+  }
+  Tensor q_out, k_out;
+  if (!out_rows(oq, *q, dev, q_out) || (k ? !out_rows(ok, *k, dev, k_out) : ok != Py_None)) return none();
+  const int64_t strides[8] = {q->stride(0), q->stride(1), k ? k->stride(0) : 0, k ? k->stride(1) : 0,
+                              q_out.stride(0), q_out.stride(1), k ? k_out.stride(0) : 0, k ? k_out.stride(1) : 0};
+  const int rc = native(nullptr, [&] {
+    return fq_rotary_embed(q->data_ptr(), k ? k->data_ptr() : nullptr, fq_dtype(dtype_code(*q)), tokens,
+                           int(q->size(1)), k ? int(k->size(1)) : 0, int(d), int(2 * freq->size(0)), strides,
+                           pos->data_ptr(), is_long(*pos), data<double>(*freq), fq_rotary_layout(layout),
+                           float(PyFloat_AS_DOUBLE(a[5])), a[6] == Py_True, q_out.data_ptr(),
+                           k ? k_out.data_ptr() : nullptr, stream_of(dev));
+  });
+  return rc == FQ_OK ? pair(q_out, k ? &k_out : nullptr) : done(rc);
+}
+
+// (q or None, key, value, key_cache, value_cache, slot_mapping, positions, frequencies, layout, scale,
+//  q_out or None)
+PyObject* rotary_append_dense(PyObject*, Args a, Py_ssize_t n) {
+  const int dev = n == 11 ? call_device(a[1]) : -1;
+  // (what is not rotated, and has no result, is left to the other path)
+  if (dev < 0 || a[0] == Py_None) return none();
+  const Tensor *q = rows(a[0], dev), *key = rows(a[1], dev), *val = rows(a[2], dev);
+  int64_t layout;
+  if (!q || !key || !val || !as_int(a[8], layout) || !PyFloat_Check(a[9])) return none();
+  const auto st = key->scalar_type();
+  const int64_t tokens = key->size(0), h = key->size(1), d = key->size(2);
+  if ((st != at::kHalf && st != at::kBFloat16) || q->scalar_type() != st || val->scalar_type() != st ||
+      val->sizes() != key->sizes() || q->size(0) != tokens || q->size(2) != d)
+    return none();
+  const Tensor *kc = pages(a[3], dev, st, true), *vc = pages(a[4], dev, st, true);
+  const Tensor *slots = ints(a[5], dev, tokens), *pos = ints(a[6], dev, tokens), *freq = frequencies(a[7], dev, d);
+  if (!kc || !vc || !slots || !pos || !freq || kc->sizes() != vc->sizes() || kc->size(2) != h || kc->size(3) != d ||
+      kc->size(1) < 1)
+    return none();
+  Tensor q_out;
+  if (!out_rows(a[10], *q, dev, q_out)) return none();
+  const int64_t strides[14] = {q->stride(0), q->stride(1), key->stride(0), key->stride(1), val->stride(0),
+                               val->stride(1), q_out.stride(0), q_out.stride(1), kc->stride(0), kc->stride(1),
+                               kc->stride(2), vc->stride(0), vc->stride(1), vc->stride(2)};
+  return done(native(nullptr, [&] {
+    return fq_rotary_append_dense(
+                  q->data_ptr(), key->data_ptr(), val->data_ptr(), fq_dtype(dtype_code(*key)), tokens,
+                  int(q->size(1)), int(h), int(d), int(2 * freq->size(0)), strides, pos->data_ptr(), is_long(*pos),
+                  data<double>(*freq), fq_rotary_layout(layout), float(PyFloat_AS_DOUBLE(a[9])), q_out.data_ptr(),
+                  kc->data_ptr(), vc->data_ptr(), int(kc->size(1)), kc->size(0) * kc->size(1), slots->data_ptr(),
+                  is_long(*slots), stream_of(dev));
+  }),
+              q_out);
+}
+
+// (q, key_cache, value_cache, block_table, seq_lens, sm_scale, window, out or None, return_lse)
+PyObject* dense_decode(PyObject*, Args a, Py_ssize_t n) {
+  const int dev = n == 9 ? call_device(a[0]) : -1;
+  if (dev < 0) return none();
+  const Tensor *q = rows(a[0], dev), *table = on_device(a[3], dev), *lens = dense(a[4], dev, at::kInt);
+  int64_t window;
+  float scale;
+  if (!q || !table || !lens || !as_int(a[6], window) || window < 0 || !PyBool_Check(a[8]) ||
+      !as_scale(a[5], q->size(2), scale))
+    return none();
+  const auto st = q->scalar_type();
+  const Tensor *kc = pages(a[1], dev, st, false), *vc = pages(a[2], dev, st, false);
+  const int64_t seqs = q->size(0), hq = q->size(1), d = q->size(2);
+  if ((st != at::kHalf && st != at::kBFloat16) || !kc || !vc || kc->sizes() != vc->sizes() || kc->size(3) != d ||
+      q->stride(0) % 2 != 0 || q->stride(1) % 2 != 0 || reinterpret_cast<uintptr_t>(q->data_ptr()) % 4 != 0 ||
+      table->dim() != 2 || table->size(0) != seqs || table->scalar_type() != at::kInt || table->stride(1) != 1 ||
+      lens->dim() != 1 || lens->size(0) != seqs || seqs > INT32_MAX || hq > INT32_MAX)
+    return none();
+  Tensor out, lse;
+  if (!decode_out(a[7], *q, dev, out)) return none();
+  if (a[7] == Py_None && !out.is_contiguous()) out = at::empty(q->sizes(), q->options());
+  if (a[8] == Py_True) lse = at::empty({seqs, hq}, q->options().dtype(at::kFloat));
+  const int hkv = int(kc->size(2));
+  const size_t need = std::max<size_t>(fq_dense_paged_decode_workspace_bytes(int(seqs), int(hq), hkv, int(d)), 32768);
+  // A call that is being recorded has a workspace of its own: two graphs that hold the stream's would share its
+  // counters when they run side by side.
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(reinterpret_cast<cudaStream_t>(stream_of(dev)), &capture) != cudaSuccess) return none();
+  std::mutex* calls = nullptr;
+  Tensor ws;
+  if (capture == cudaStreamCaptureStatusNone) {
+    ws = workspace(dev, kDense, need, &calls);
+  } else {
+    ws = call_bytes(dev, need, false);
+    ws.narrow(0, 0, 32768).zero_();
+  }
+  const int rc = native(calls, [&] {
+    return fq_dense_paged_decode(
+        q->data_ptr(), fq_dtype(dtype_code(*q)), q->stride(0), q->stride(1), kc->data_ptr(), kc->stride(0),
+        kc->stride(1), kc->stride(2), vc->data_ptr(), vc->stride(0), vc->stride(1), vc->stride(2),
+        data<int32_t>(*table), table->stride(0), int(table->size(1)), data<int32_t>(*lens), int(seqs), int(hq), hkv,
+        int(d), int(kc->size(1)), kc->size(0), scale, int(window), out.data_ptr(),
+        lse.defined() ? data(lse) : nullptr, ws.data_ptr(), size_t(ws.numel()), stream_of(dev));
+  });
+  if (rc != FQ_OK || !lse.defined()) return done(rc, out);
+  return pair(out, &lse);
+}
+
+struct Pool {
+  const Tensor *table, *free, *count;
+  Tensor count_out;
+  int64_t requests, width, stride, block_size;
+};
+bool pool_args(PyObject* table, PyObject* free, PyObject* count, PyObject* block_size, PyObject* out, int dev, Pool& p) {
+  p.table = on_device(table, dev);
+  p.free = dense(free, dev, at::kInt);
+  p.count = dense(count, dev, at::kInt);
+  if (!p.table || !p.free || !p.count || p.table->dim() != 2 || p.table->scalar_type() != at::kInt ||
+      p.table->stride(1) != 1 || p.free->dim() != 1 || p.count->numel() != 1 || !as_int(block_size, p.block_size) ||
+      p.block_size < 1)
+    return false;
+  p.requests = p.table->size(0);
+  p.width = p.table->size(1);
+  p.stride = std::max(p.table->stride(0), p.width);
+  if (p.requests > INT32_MAX || p.width > INT32_MAX || (p.requests > 1 && p.table->stride(0) < p.width)) return false;
+  if (out == Py_None) {
+    p.count_out = at::empty({1}, p.count->options());
+    return true;
+  }
+  const Tensor* t = dense(out, dev, at::kInt);
+  if (!t || t->numel() != 1) return false;
+  p.count_out = *t;
+  return true;
+}
+
+// (context_lens, query_lens, block_table, free_blocks, free_count, block_size, max_tokens, free_count_out or None)
+PyObject* plan_paged_step(PyObject*, Args a, Py_ssize_t n) {
+  const int dev = n == 8 ? call_device(a[2]) : -1;
+  if (dev < 0) return none();
+  Pool p;
+  int64_t room;
+  if (!as_int(a[6], room) || room < 0 || !pool_args(a[2], a[3], a[4], a[5], a[7], dev, p)) return none();
+  const Tensor *context = dense(a[0], dev, at::kInt), *query = dense(a[1], dev, at::kInt);
+  if (!context || !query || context->dim() != 1 || query->dim() != 1 || context->size(0) != p.requests ||
+      query->size(0) != p.requests)
+    return none();
+  const auto i32 = p.table->options(), i64 = i32.dtype(at::kLong);
+  const Tensor out[6] = {at::empty({p.requests}, i32), at::empty({p.requests + 1}, i32), at::empty({room}, i64),
+                         at::empty({room}, i64), at::empty({p.requests}, i32.dtype(at::kBool)), p.count_out};
+  const int rc = native(nullptr, [&] {
+    return fq_plan_paged_step(data<int32_t>(*context), data<int32_t>(*query), int(p.requests), data<int32_t>(*p.table),
+                              p.stride, int(p.width), int(p.block_size), data<int32_t>(*p.free), p.free->numel(),
+                              data<int32_t>(*p.count), room, data<int32_t>(out[0]), data<int32_t>(out[1]),
+                              data<int64_t>(out[2]), data<int64_t>(out[3]), data<uint8_t>(out[4]),
+                              data<int32_t>(out[5]), stream_of(dev));
+  });
+  if (rc != FQ_OK) return done(rc);
+  PyObject* t = PyTuple_New(6);
+  for (int i = 0; t && i < 6; ++i) PyTuple_SET_ITEM(t, i, THPVariable_Wrap(out[i]));
+  return t;
+}
+
+// (finished, context_lens, block_table, free_blocks, free_count, block_size, free_count_out or None)
+PyObject* release_pages(PyObject*, Args a, Py_ssize_t n) {
+  const int dev = n == 7 ? call_device(a[2]) : -1;
+  if (dev < 0) return none();
+  Pool p;
+  if (!pool_args(a[2], a[3], a[4], a[5], a[6], dev, p)) return none();
+  const Tensor *finished = dense(a[0], dev, at::kBool), *context = dense(a[1], dev, at::kInt);
+  if (!finished || !context || finished->dim() != 1 || context->dim() != 1 || finished->size(0) != p.requests ||
+      context->size(0) != p.requests)
+    return none();
+  return done(native(nullptr, [&] {
+    return fq_release_pages(data<uint8_t>(*finished), data<int32_t>(*context), int(p.requests),
+                            data<int32_t>(*p.table), p.stride, int(p.width), int(p.block_size),
+                            data<int32_t>(*p.free), p.free->numel(), data<int32_t>(*p.count),
+                            data<int32_t>(p.count_out), stream_of(dev));
+  }),
+              p.count_out);
+}
+
 // C++ exceptions (an allocation that fails) become Python ones
 PyObject* g_oom = nullptr;  // torch.OutOfMemoryError
 template <PyObject* (*F)(PyObject*, Args, Py_ssize_t)>
@@ -573,6 +816,8 @@ PyMethodDef kMethods[] = {
     FQ_METHOD(compress_append), FQ_METHOD(compress_append_qjl), FQ_METHOD(paged_decode),
     FQ_METHOD(paged_decode_qjl), FQ_METHOD(paged_decode_multi), FQ_METHOD(paged_prefill),
     FQ_METHOD(compress), FQ_METHOD(attention), FQ_METHOD(cache_update),
+    FQ_METHOD(rotary_embed), FQ_METHOD(rotary_append_dense), FQ_METHOD(dense_decode),
+    FQ_METHOD(plan_paged_step), FQ_METHOD(release_pages),
     {"workspaces", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&py_workspaces)),
      METH_FASTCALL, nullptr},
     {"workspace", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&py_workspace)),

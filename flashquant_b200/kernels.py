@@ -422,7 +422,7 @@ def tq4_compress_append_qjl(key, value, kv_cache, kq_cache, slot_mapping, rotati
 # --------------------------------------------------------------------------------------
 
 # uses of the cached workspaces (one per device, stream and use)
-_DECODE, _ATTENTION = 0, 1
+_DECODE, _ATTENTION, _DENSE = 0, 1, 2
 
 
 def _workspace(device, use: int, need: int) -> torch.Tensor:

@@ -598,6 +598,106 @@ int fq_decode_step_host_packed(const void* block_host, void* out_host, int overl
                                void* staging, size_t staging_bytes, void* workspace,
                                size_t workspace_bytes, fq_stream_t stream);
 
+/*
+ * Block tables, slots and positions of a step, from the lengths of its requests (one launch).
+ * What a scheduler fills in on the host for FlashQuantAttentionMetadata (block table, slot
+ * mapping, sequence lengths, query starts: src/flashquant/vllm/impl.py:220-263, 362-395).
+ *   context_lens   num_requests: tokens of a request that are in the cache
+ *   query_lens     num_requests: its new tokens
+ *   block_table    (num_requests, block_table_width) of row stride block_table_stride; the pages
+ *                  of the cached tokens stand in it, those of the new tokens are written behind
+ *   free_blocks    a stack of free pages (free_capacity entries, the first *free_count of them in
+ *                  use); requests take from its top, in order
+ *   max_tokens     entries of slot_mapping and positions
+ * Out: seq_lens (context + new), cu_seqlens_q (num_requests + 1), slot_mapping and positions of the
+ * new tokens (-1 behind the last), served (1 byte a request), *free_count_out (may be free_count).
+ * A request is served if the stack holds the pages, and slot_mapping the tokens, of all requests up
+ * to and including it; one without new tokens always is.  A negative length, or more pages than a
+ * row holds, is not served and takes nothing.  At most 4096 requests.
+ */
+int fq_plan_paged_step(const int32_t* context_lens, const int32_t* query_lens, int num_requests,
+                       int32_t* block_table, int64_t block_table_stride, int block_table_width,
+                       int block_size, const int32_t* free_blocks, int64_t free_capacity,
+                       const int32_t* free_count, int64_t max_tokens, int32_t* seq_lens,
+                       int32_t* cu_seqlens_q, int64_t* slot_mapping, int64_t* positions,
+                       uint8_t* served, int32_t* free_count_out, fq_stream_t stream);
+/* The way back: the pages of the requests with finished[i] != 0 (ceil(context_lens[i] /
+ * block_size) entries of their rows) go on the stack, in order; what is beyond free_capacity is
+ * dropped. */
+int fq_release_pages(const uint8_t* finished, const int32_t* context_lens, int num_requests,
+                     const int32_t* block_table, int64_t block_table_stride, int block_table_width,
+                     int block_size, int32_t* free_blocks, int64_t free_capacity,
+                     const int32_t* free_count, int32_t* free_count_out, fq_stream_t stream);
+
+/* Which values of a head make a pair: x[j] and x[j + rotary_dim / 2], or x[2j] and x[2j + 1]. */
+typedef enum fq_rotary_layout {
+  FQ_ROTARY_HALF = 0,
+  FQ_ROTARY_INTERLEAVED = 1
+} fq_rotary_layout;
+
+/*
+ * Rotary positions: pair j of every head of token i is turned by positions[i] * frequencies[j]
+ * (taken in 64 bits) and multiplied by `scale`; values from rotary_dim on are copied.
+ *   q, k           (tokens, heads, head_dim) of `dtype`; a null k with num_k_heads = 0 is left out
+ *   strides        in elements: q token, q head, k token, k head, q_out token, q_out head,
+ *                  k_out token, k_out head; the values of a head are adjacent
+ *   frequencies    rotary_dim / 2, fp64
+ *   inverse        turns by the negative angle (with the same scale: the transposed map, which
+ *                  takes gradients, or keys, back)
+ * q_out and k_out may be q and k.  Tokens with a negative position are not written.
+ */
+int fq_rotary_embed(const void* q, const void* k, fq_dtype dtype, int64_t tokens, int num_q_heads,
+                    int num_k_heads, int head_dim, int rotary_dim, const int64_t* strides,
+                    const void* positions, int positions_are_int64, const double* frequencies,
+                    fq_rotary_layout layout, float scale, int inverse, void* q_out, void* k_out,
+                    fq_stream_t stream);
+
+/*
+ * Append to pages of 16-bit keys and values (fp16 or bf16), rotary positions on the way: q goes to
+ * q_out, the keys of token i to row slot_mapping[i] of key_cache, its values to that of
+ * value_cache.  A slot outside [0, num_slots) stores nothing; rotary_dim = 0 appends as it is.
+ *   strides        q token, q head, key token, key head, value token, value head, q_out token,
+ *                  q_out head, then block, token, head of key_cache and of value_cache
+ * A slot is block * block_size + token, as in fq_tq4_compress_append.
+ */
+int fq_rotary_append_dense(const void* q, const void* key, const void* value, fq_dtype dtype,
+                           int64_t tokens, int num_q_heads, int num_kv_heads, int head_dim,
+                           int rotary_dim, const int64_t* strides, const void* positions,
+                           int positions_are_int64, const double* frequencies,
+                           fq_rotary_layout layout, float scale, void* q_out, void* key_cache,
+                           void* value_cache, int block_size, int64_t num_slots,
+                           const void* slot_mapping, int slots_are_int64, fq_stream_t stream);
+
+/*
+ * Attention of one query token per sequence over pages of 16-bit keys and values: the layers of a
+ * model whose cache is not compressed, over the block tables of those that are
+ * (fq_split_k_paged_decode).  One launch, split over the tokens and joined in it.
+ *   q              (num_seqs, num_q_heads, head_dim), strides in elements
+ *   key_cache,     row (block, token, head) at block * *_block_stride + token * *_token_stride +
+ *   value_cache    head * *_head_stride; rows start at multiples of 16 bytes
+ *   window         each sequence sees its last `window` tokens (0: all)
+ *   out            contiguous like q; zeros for a sequence without tokens
+ *   lse            optional (num_seqs, num_q_heads): the natural logarithm of the sum of
+ *                  exp(sm_scale q k); -inf without tokens
+ *   workspace      fq_dense_paged_decode_workspace_bytes(...), 16-byte aligned, one per
+ *                  concurrent call; its first 32 KiB zero before its first use
+ * head_dim 64, 96, 128 or 256; block_size a multiple of 16; any number of query heads per KV head.
+ * Keys and values of visible tokens are finite; what stands in other rows does not matter.
+ * Status word (word 0): FQ_DEV_BAD_BLOCK_INDEX where a page id was out of range, or a length beyond
+ * the block-table row (the page is skipped, the length cut).
+ */
+size_t fq_dense_paged_decode_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads,
+                                             int head_dim);
+int fq_dense_paged_decode(const void* q, fq_dtype dtype, int64_t q_seq_stride,
+                          int64_t q_head_stride, const void* key_cache, int64_t k_block_stride,
+                          int64_t k_token_stride, int64_t k_head_stride, const void* value_cache,
+                          int64_t v_block_stride, int64_t v_token_stride, int64_t v_head_stride,
+                          const int32_t* block_table, int64_t block_table_stride,
+                          int block_table_width, const int32_t* seq_lens, int num_seqs,
+                          int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                          int64_t num_blocks, float sm_scale, int window, void* out, float* lse,
+                          void* workspace, size_t workspace_bytes, fq_stream_t stream);
+
 /* Copies the device status word of a decode workspace to *status (synchronises stream). */
 int fq_workspace_status(const void* workspace, uint32_t* status, fq_stream_t stream);
 
