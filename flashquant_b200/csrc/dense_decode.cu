@@ -8,11 +8,16 @@
 //
 // Every warp streams on its own: a ring of tiles of 16 tokens in shared memory, filled by cp.async (16 bytes a
 // lane, rows outside the sequence filled with zeros), no barrier of the CTA in the loop.  How the tiles are dealt
-// out: dense_split.h.  Sums, maxima and weights are fp32; a weight enters the value product as two 16-bit terms
-// (hi + lo, 2^-17 of it or better), so that the output is rounded once, at the end.  With up to eight query heads
-// per unit the lo terms are the rows 8..15 of the A operand and cost nothing.
+// out: dense_split.h.  Sixteen lanes find what the next sixteen tiles are and where they stand (the page's id on its
+// way while earlier tiles are worked on) and leave that in shared memory.  Sums, maxima and weights are fp32; a
+// weight enters the value product as two 16-bit terms (hi + lo, 2^-17 of it or better), so that the output is
+// rounded once, at the end.  With up to eight query heads per unit the lo terms are the rows 8..15 of the A operand
+// and cost nothing.
+//
+// What is left in pieces is joined by a second kernel, launched with the first (programmatic dependent launch): a
+// CTA per query head, pieces in the order of the list.  Joined by the last warp to arrive, behind fences and a
+// counter, 1 x 900 tokens took 20 us, and one warp had to read all pieces of a long sequence.
 #include <algorithm>
-#include <type_traits>
 
 #include "dense_split.h"
 #include "fq_common.cuh"
@@ -21,9 +26,10 @@ namespace fq {
 
 constexpr int kDenseMaxCtas = 148;
 constexpr int kDenseMaxSeqs = 2048;
-constexpr size_t kDenseHead = 32768;     // status word, counters (zero between calls); then the pieces
-constexpr size_t kDenseCounters = 256;   // [CTA][warp]
-constexpr int kDenseShortest = 4;        // tiles to a run at least
+// Workspace: the head (status word; the number of runs taken), zero between calls; the list's bounds of the
+// sequences; pieces.
+constexpr size_t kDenseTickets = 64, kDenseBounds = 32768, kDensePieces = kDenseBounds + 16384;
+static_assert((kDenseMaxSeqs + 1) * sizeof(int) <= kDensePieces - kDenseBounds, "");
 
 struct DenseArgs {
   const void *q, *k, *v;
@@ -37,20 +43,28 @@ struct DenseArgs {
   int chunks, rows;                      // units of a KV head, query heads of a unit
   int side, piece_floats;                // units side by side; stride of the pieces
   float scale_log2;
-  uint32_t* status;
-  uint32_t* counters;
-  float* pieces;
+  int fixed;                             // runs dealt out beforehand
+  uint32_t *status, *tickets;
+  int* bounds;
+  float* pieces;                         // [run][side][slot]: [rows][D], [rows][2] (maximum, sum)
 };
+
+// Warps of a CTA, one CTA per SM: as many as the registers leave (a row of the accumulators is D floats).  head_dim 64,
+// 48 x 1000 tokens: ... us with 8, ... with 16.
+__host__ __device__ constexpr int dense_warps(int d) { return d == 64 ? 16 : (d > 128 ? 4 : 8); }
 
 template <int D>
 struct DenseShape {
-  static constexpr int kWarps = D > 128 ? 4 : 8;
-  static constexpr int kPitch = 2 * D + 16;  // bytes of a row: 16 beyond it, so that 8 rows fall into all banks
-  static constexpr int kTensor = kDenseTile * kPitch;
+  static constexpr int kWarps = dense_warps(D);
+  static constexpr int kRow = 2 * D;         // bytes
+  static constexpr int kTensor = kDenseTile * kRow;
   static constexpr int kStage = 2 * kTensor;
-  static constexpr int kStages = D == 64 ? 5 : (D == 96 ? 4 : 3);
+  static constexpr int kStages = D == 96 ? 4 : 3;  // 192 KB in all
   static constexpr int kRing = kStages * kStage;
-  static constexpr int kSmem = kWarps * kRing;
+  static constexpr int kDescribed = kWarps * 32 * 16;  // 32 tiles of a warp
+  static constexpr int kSmem = kWarps * kRing + kDescribed;
+  // The 16-byte chunks of a row are permuted, so that the same chunk of 8 rows stands in all banks.
+  static __device__ __forceinline__ int key(int row) { return D == 96 ? row >> 1 & 3 : row & 7; }
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
@@ -104,23 +118,30 @@ struct Dense16<__nv_bfloat16> {
   }
 };
 
-// Where a warp stands in the list of tiles.
-struct DenseCursor {
-  int at, end;        // entries of its run
-  int a, b;           // entries of the unit group
-  int seq, group;     // the sequence, its unit group
-  int begin, len;     // tokens seen: [begin, len)
-  int tile;           // of the sequence
+// A tile: x the page (-1: none), y the first token in it | first visible row << 22 | row behind the last << 26,
+// z sequence | unit << 12 | first of the unit << 30 | last << 31 (of what this run has of it), w the piece (-1: all
+// of the unit is here).
+constexpr int kDenseMaxBlock = 1 << 22;
+
+struct DenseUnit {
+  int head0, count;  // query heads
 };
+__device__ __forceinline__ DenseUnit dense_unit(const DenseArgs& p, int unit) {
+  const int group = p.hq / p.hkv, kv = unit / p.chunks, chunk = unit - kv * p.chunks;
+  return {kv * group + chunk * p.rows, min(p.rows, group - chunk * p.rows)};
+}
+__device__ __forceinline__ float dense_lse(float m, float l, float lift) {
+  return l == 0.f ? -INFINITY : (m + log2f(l) - lift) * 0.69314718f;
+}
 
 template <typename T, int D, bool R16>
 __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_kernel(const DenseArgs p) {
   using S = DenseShape<D>;
   using X = Dense16<T>;
-  constexpr int kRows = R16 ? 16 : 8;
   constexpr int kSteps = D / 16, kBlocks = D / 8;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int warp_total[S::kWarps];
+  int4* const described = reinterpret_cast<int4*>(smem + S::kWarps * S::kRing);
   int* const prefix = reinterpret_cast<int*>(smem + S::kSmem);  // [seqs + 1]
   int* const lengths = prefix + p.seqs + 1;                     // [seqs]
   const int tid = threadIdx.x, lane = tid & 31;
@@ -128,6 +149,7 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
   const int g = lane >> 2, t = lane & 3;
   const int64_t room = int64_t(p.table_width) * p.block_size;
   const int unit_groups = p.hkv * p.chunks / p.side;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // ---- the list: prefix sums of the sequences' tiles -------------------------------------------------
   {
@@ -153,94 +175,108 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
     __syncthreads();
     for (int w = 0; w < warp; ++w) before += warp_total[w];
     if (tid == 0) prefix[0] = 0;
-    for (int s = s0; s < s1; ++s) prefix[s + 1] += before;
+    for (int s = s0; s < s1; ++s) {
+      prefix[s + 1] += before;
+      if (blockIdx.x == 0) p.bounds[s + 1] = prefix[s + 1];
+    }
+    if (blockIdx.x == 0 && tid == 0) p.bounds[0] = 0;
     __syncthreads();
   }
-  const int teams = S::kWarps / p.side;
-  const int team = warp / p.side, member = warp - team * p.side;
-  const DenseCut cut = dense_cut(prefix[p.seqs], gridDim.x, teams, kDenseShortest);
+  const DenseCut cut = dense_cut(prefix[p.seqs], p.fixed);
 
-  // rows of sequences without a token
-  for (int s = blockIdx.x; s < p.seqs; s += gridDim.x) {
-    if (prefix[s + 1] != prefix[s]) continue;
-    uint32_t* o = static_cast<uint32_t*>(p.out) + int64_t(s) * p.hq * (D / 2);
-    for (int i = tid; i < p.hq * (D / 2); i += S::kWarps * 32) o[i] = 0u;
-    if (p.lse)
-      for (int i = tid; i < p.hq; i += S::kWarps * 32) p.lse[int64_t(s) * p.hq + i] = -INFINITY;
-  }
-
-  // ---- cursors ----------------------------------------------------------------------------------------
-  auto enter = [&](DenseCursor& c) {  // c.seq, c.group -> the other fields, at the unit group's first entry
-    c.len = lengths[c.seq];
-    const DenseSpan span = dense_span(c.len, room, p.window);
-    c.begin = span.begin;
-    c.a = prefix[c.seq] + c.group * span.tiles;
-    c.b = c.a + span.tiles;
-    c.tile = span.first_tile;
-  };
-  auto start = [&](DenseCursor& c, int run) {
-    c.at = cut.begin(run);
-    c.end = cut.end(run);
-    if (c.at >= c.end) return;
-    int lo = 0, hi = p.seqs - 1;  // the sequence whose entries hold c.at
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (prefix[mid + 1] > c.at) hi = mid; else lo = mid + 1;
-    }
-    c.seq = lo;
-    const int tiles = (prefix[lo + 1] - prefix[lo]) / unit_groups;
-    c.group = (c.at - prefix[lo]) / tiles;
-    enter(c);
-    c.tile += c.at - c.a;
-  };
-  auto advance = [&](DenseCursor& c) {
-    ++c.at;
-    ++c.tile;
-    if (c.at < c.b || c.at >= c.end) return;
-    if (++c.group == unit_groups) {
-      c.group = 0;
-      do ++c.seq; while (prefix[c.seq + 1] == prefix[c.seq]);
-    }
-    enter(c);
-  };
-
-  const int run = blockIdx.x * teams + team;
-  const uint32_t ring = smem_u32(smem) + warp * S::kRing;
+  // ---- the warp's tiles, described sixteen at a time ---------------------------------------------------
   const int tiles_per_block = p.block_size / kDenseTile;
-
-  DenseCursor ld;
-  start(ld, run);
-  DenseCursor cu = ld;
-  int block = 0;  // the page of ld's tile (loaded a tile ahead of its use)
-  auto look_up = [&] {
-    if (ld.at < ld.end) block = p.table[ld.seq * p.table_stride + ld.tile / tiles_per_block];
+  const uint32_t taken = uint32_t(cut.taken()) * p.side;
+  int4* const mine = described + warp * 32;
+  const int here = blockIdx.x * S::kWarps + warp;
+  int run = here / p.side, member = here - run * p.side;
+  int at = cut.begin(run), end = cut.end(run);
+  uint32_t ticket = 0;  // (lane 0) the next run
+  auto take = [&] {
+    if (taken && lane == 0) ticket = atomicAdd(p.tickets, 1u);
   };
-  look_up();
-  uint32_t bad = 0;  // bit i: stage i holds a tile whose page does not exist
+  take();
+  int made = 0, issued = 0, used = 0;  // tiles described, on their way, done
+  int waiting = 0;                     // described in `next`, not stored yet
+  bool finished = false;
+  int4 next;
+  auto describe = [&] {
+    if (at == end) {
+      uint32_t x = __shfl_sync(0xffffffffu, ticket, 0);
+      if (x >= taken) {
+        // (every warp gets one that is too large: the last of them leaves the counter as it was found)
+        if (taken && lane == 0 && x == taken + gridDim.x * S::kWarps - 1) *p.tickets = 0u;
+        finished = true;
+        return;
+      }
+      run = cut.fixed + x / p.side;
+      member = x % p.side;
+      at = cut.begin(run);
+      end = cut.end(run);
+      take();
+    }
+    waiting = min(16, end - at);
+    if (lane < waiting) {
+      const int here = at + lane;
+      int lo = 0, hi = p.seqs - 1;  // the sequence whose entries hold `here`
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (prefix[mid + 1] > here) hi = mid; else lo = mid + 1;
+      }
+      const DenseSpan span = dense_span(lengths[lo], room, p.window);
+      const int group = (here - prefix[lo]) / span.tiles;
+      const int a = prefix[lo] + group * span.tiles, b = a + span.tiles;
+      const int tile = span.first_tile + here - a;
+      const int page = tile / tiles_per_block, first = tile * kDenseTile;
+      next.x = __ldg(p.table + lo * p.table_stride + page);
+      next.y = (tile - page * tiles_per_block) * kDenseTile | max(span.begin - first, 0) << 22 |
+               min(span.len - first, kDenseTile) << 26;
+      next.z = lo | (group * p.side + member) << 12;
+      if (here == a || here == cut.begin(run)) next.z |= 1 << 30;
+      if (here + 1 == b || here + 1 == end) next.z |= 1 << 31;
+      next.w = a >= cut.begin(run) && b <= end ? -1 : (run * p.side + member) * 2 + dense_slot(cut, run, a);
+    }
+    at += waiting;
+  };
+  auto store = [&] {
+    if (lane < waiting) {
+      if (unsigned(next.x) >= uint64_t(p.num_blocks)) {
+        next.x = -1;
+        atomicOr(p.status, FQ_DEV_BAD_BLOCK_INDEX);
+      }
+      mine[(made + lane) & 31] = next;
+    }
+    made += waiting;
+    waiting = 0;
+    __syncwarp();
+  };
+
+  const uint32_t ring = smem_u32(smem) + warp * S::kRing;
+  constexpr int kPerRow = D / 8, kChunks = kDenseTile * kPerRow / 32;
+  // one tile on its way, if there is one (each call is a group: tile n is complete when group n is)
   auto issue = [&](int stage) {
-    if (ld.at < ld.end) {
-      const bool ok = unsigned(block) < uint64_t(p.num_blocks);
-      bad = ok ? bad & ~(1u << stage) : bad | (1u << stage);
-      const int first = ld.tile * kDenseTile;
-      const int head = (ld.group * p.side + member) / p.chunks;
-      const int64_t id = ok ? block : 0;
-      const int row = (ld.tile % tiles_per_block) * kDenseTile;
+    while (issued == made && !finished) {
+      if (!waiting) describe();
+      store();
+    }
+    if (issued < made) {
+      const int4 d = mine[issued & 31];
+      ++issued;
+      const int head = ((d.z >> 12) & 0x3fff) / p.chunks;
+      const int row = d.y & (kDenseMaxBlock - 1);
+      const int64_t id = d.x < 0 ? 0 : d.x;
       const T* k = static_cast<const T*>(p.k) + id * p.k_block + row * p.k_token + head * p.k_head;
       const T* v = static_cast<const T*>(p.v) + id * p.v_block + row * p.v_token + head * p.v_head;
-      const int lo = ld.begin - first, hi = ok ? ld.len - first : 0;
+      const int lo = (d.y >> 22) & 15, hi = d.x < 0 ? 0 : (d.y >> 26) & 31;
       const uint32_t dst = ring + stage * S::kStage;
-      constexpr int kPerRow = D / 8;
 #pragma unroll
-      for (int c = 0; c < kDenseTile * kPerRow / 32; ++c) {
+      for (int c = 0; c < kChunks; ++c) {
         const int i = lane + 32 * c, r = i / kPerRow, col = i % kPerRow;
         const bool valid = r >= lo && r < hi;
-        const int64_t rr = valid ? r : 0;
-        cp_async16(dst + r * S::kPitch + col * 16, k + (valid ? rr * p.k_token + col * 8 : 0), valid);
-        cp_async16(dst + S::kTensor + r * S::kPitch + col * 16, v + (valid ? rr * p.v_token + col * 8 : 0),
-                   valid);
+        const uint32_t to = dst + r * S::kRow + ((col ^ S::key(r)) << 4);
+        cp_async16(to, k + (valid ? r * p.k_token + col * 8 : 0), valid);
+        cp_async16(to + S::kTensor, v + (valid ? r * p.v_token + col * 8 : 0), valid);
       }
-      advance(ld);
-      look_up();
     }
     cp_async_commit();
   };
@@ -250,19 +286,12 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
   float acc[kBlocks][4];
   float top[R16 ? 2 : 1], sum[R16 ? 2 : 1];
 
-  auto unit_heads = [&](const DenseCursor& c, int& head0, int& count) {
-    const int unit = c.group * p.side + member, group = p.hq / p.hkv;
-    const int kv = unit / p.chunks, chunk = unit - kv * p.chunks;
-    head0 = kv * group + chunk * p.rows;
-    count = min(p.rows, group - chunk * p.rows);
-  };
-  auto begin_unit = [&] {
-    int head0, count;
-    unit_heads(cu, head0, count);
-    const T* q = static_cast<const T*>(p.q) + cu.seq * p.q_seq + head0 * p.q_head;
+  auto begin_unit = [&](const int4& d) {
+    const DenseUnit u = dense_unit(p, (d.z >> 12) & 0x3fff);
+    const T* q = static_cast<const T*>(p.q) + (d.z & 0xfff) * p.q_seq + u.head0 * p.q_head;
 #pragma unroll
     for (int r = 0; r < (R16 ? 2 : 1); ++r) {
-      const bool real = g + 8 * r < count;
+      const bool real = g + 8 * r < u.count;
       const T* row = q + (real ? (g + 8 * r) * p.q_head : 0) + 2 * t;
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
@@ -278,16 +307,17 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
     for (int j = 0; j < kBlocks; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
   };
 
-  auto tile_step = [&](int stage) {
+  auto tile_step = [&](int stage, const int4& d) {
     const uint32_t kt = ring + stage * S::kStage, vt = kt + S::kTensor;
     const int mid = lane >> 3;
     // scores: rows = heads, columns = tokens (two blocks of eight)
     float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    const uint32_t ka = kt + ((mid >> 1) * 8 + (lane & 7)) * S::kPitch + (mid & 1) * 16;
+    const int k_row = (mid >> 1) * 8 + (lane & 7), v_row = (mid & 1) * 8 + (lane & 7);
+    const uint32_t ka = kt + k_row * S::kRow, k_key = ((mid & 1) ^ S::key(k_row)) << 4;
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
       uint32_t b[4];
-      ldmatrix4(b, ka + i * 32);
+      ldmatrix4(b, ka + (i * 32 ^ k_key));
       uint32_t a[4];
       if constexpr (R16) {
         a[0] = qf[i][0]; a[1] = qf[i][1]; a[2] = qf[i][2]; a[3] = qf[i][3];
@@ -301,8 +331,7 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[n][e] *= p.scale_log2;
-    const int first = cu.tile * kDenseTile;
-    const int lo = cu.begin - first, hi = (bad >> stage) & 1 ? 0 : cu.len - first;
+    const int lo = (d.y >> 22) & 15, hi = d.x < 0 ? 0 : (d.y >> 26) & 31;
     if (lo > 0 || hi < kDenseTile) {
 #pragma unroll
       for (int n = 0; n < 2; ++n)
@@ -352,11 +381,11 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
         }
       }
     }
-    const uint32_t va = vt + ((mid & 1) * 8 + (lane & 7)) * S::kPitch + (mid >> 1) * 16;
+    const uint32_t va = vt + v_row * S::kRow, v_key = ((mid >> 1) ^ S::key(v_row)) << 4;
 #pragma unroll
     for (int j = 0; j < kBlocks; j += 2) {
       uint32_t b[4];
-      ldmatrix4_trans(b, va + j * 16);
+      ldmatrix4_trans(b, va + (j * 16 ^ v_key));
       X::mma(acc[j], hi_a, b[0], b[1]);
       X::mma(acc[j + 1], hi_a, b[2], b[3]);
       if constexpr (R16) {
@@ -366,28 +395,19 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
     }
   };
 
-  // ---- results ----------------------------------------------------------------------------------------
-  auto piece_of = [&](int run_, int slot) {
-    return p.pieces + ((int64_t(run_) * p.side + member) * 2 + slot) * p.piece_floats;
-  };
-  auto write_pair = [&](int seq, int head, int dim, float x, float y) {
-    *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (int64_t(seq) * p.hq + head) * D + dim) = X::pack(x, y);
-  };
-  auto write_lse = [&](int seq, int head, float m, float l) {
-    if (p.lse)
-      p.lse[int64_t(seq) * p.hq + head] = l == 0.f ? -INFINITY : (m + log2f(l) - X::kLift) * 0.69314718f;
-  };
-  // the warp's unit: to `out` (dst null), or as a piece [rows][D], [rows][2] (maximum, sum)
-  auto flush = [&](float* dst) {
-    int head0, count;
-    unit_heads(cu, head0, count);
+  // the unit, or what the run has of it: to `out`, or as a piece
+  auto flush = [&](const int4& d) {
+    const int seq = d.z & 0xfff;
+    const DenseUnit u = dense_unit(p, (d.z >> 12) & 0x3fff);
+    float* const dst = p.pieces + int64_t(d.w) * p.piece_floats;
 #pragma unroll
     for (int r = 0; r < (R16 ? 2 : 1); ++r) {
       float l = sum[r];
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       l += __shfl_xor_sync(0xffffffffu, l, 2);
       const int row = g + 8 * r;
-      if (row >= count) continue;
+      if (row >= u.count) continue;
+      const int64_t out_row = int64_t(seq) * p.hq + u.head0 + row;
       const float f = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
       for (int j = 0; j < kBlocks; ++j) {
@@ -396,179 +416,169 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
           x += acc[j][2];
           y += acc[j][3];
         }
-        if (dst)
+        if (d.w >= 0)
           *reinterpret_cast<float2*>(dst + row * D + 8 * j + 2 * t) = make_float2(x, y);
         else
-          write_pair(cu.seq, head0 + row, 8 * j + 2 * t, x * f, y * f);
+          *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + out_row * D + 8 * j + 2 * t) = X::pack(x * f, y * f);
       }
       if (t == 0) {
-        if (dst)
+        if (d.w >= 0)
           *reinterpret_cast<float2*>(dst + p.rows * D + 2 * row) = make_float2(top[r], l);
-        else
-          write_lse(cu.seq, head0 + row, top[r], l);
+        else if (p.lse)
+          p.lse[out_row] = dense_lse(top[r], l, X::kLift);
       }
     }
-  };
-
-  // Joins n pieces (piece(i): the i-th; SHARED: in shared memory, else in the workspace) into `out` or one
-  // piece.  32 at a time: lane r finds the weights of row r and leaves them in the warp's part of shared memory,
-  // then every lane sums its columns of four dimensions.
-  float* const weights = reinterpret_cast<float*>(smem + warp * S::kRing);  // [33][kRows]
-  float* const meet = weights + 33 * kRows;                                 // a piece, of a merging CTA
-  auto join = [&](auto shared, const DenseCursor& c, int n, auto piece, float* dst) {
-    constexpr bool kShared = decltype(shared)::value;
-    auto load2 = [](const float* x) {
-      const float2* y = reinterpret_cast<const float2*>(x);
-      if constexpr (kShared) return *y; else return __ldcg(y);
-    };
-    auto load4 = [](const float* x) {
-      const float4* y = reinterpret_cast<const float4*>(x);
-      if constexpr (kShared) return *y; else return __ldcg(y);
-    };
-    int head0, count;
-    unit_heads(c, head0, count);
-    constexpr int kVecs = kRows * D / 4 / 32;  // columns of a lane
-    float4 o[kVecs];
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    float m = -INFINITY, l = 0.f;  // of row `lane`
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      const int some = min(32, n - i0);
-      __syncwarp();
-      if (lane < count) {
-        float now = m;
-        for (int i = 0; i < some; ++i) now = fmaxf(now, load2(piece(i0 + i) + p.rows * D + 2 * lane).x);
-        const float ref = now == -INFINITY ? 0.f : now;
-        const float f = fast_exp2(m - ref);
-        l *= f;
-        for (int i = 0; i < some; ++i) {
-          const float2 x = load2(piece(i0 + i) + p.rows * D + 2 * lane);
-          const float w = fast_exp2(x.x - ref);
-          l = fmaf(w, x.y, l);
-          weights[i * kRows + lane] = w;
-        }
-        m = now;
-        weights[32 * kRows + lane] = f;
-      }
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < kVecs; ++i) {
-        const int row = (lane + 32 * i) * 4 / D;
-        const float f = row < count ? weights[32 * kRows + row] : 0.f;
-        o[i].x *= f; o[i].y *= f; o[i].z *= f; o[i].w *= f;
-      }
-#pragma unroll 4
-      for (int k = 0; k < some; ++k) {
-        const float* src = piece(i0 + k);
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-          const int row = (lane + 32 * i) * 4 / D;
-          if (row < count) {
-            const float w = weights[k * kRows + row];
-            const float4 x = load4(src + 4 * (lane + 32 * i));
-            o[i].x = fmaf(w, x.x, o[i].x);
-            o[i].y = fmaf(w, x.y, o[i].y);
-            o[i].z = fmaf(w, x.z, o[i].z);
-            o[i].w = fmaf(w, x.w, o[i].w);
-          }
-        }
-      }
-    }
-    __syncwarp();
-    if (lane < count) {
-      if (dst)
-        *reinterpret_cast<float2*>(dst + p.rows * D + 2 * lane) = make_float2(m, l);
-      else
-        write_lse(c.seq, head0 + lane, m, l);
-      weights[lane] = l == 0.f ? 0.f : 1.f / l;
-    }
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      const int row = (lane + 32 * i) * 4 / D, dim = (lane + 32 * i) * 4 % D;
-      if (row >= count) continue;
-      if (dst) {
-        reinterpret_cast<float4*>(dst)[lane + 32 * i] = o[i];
-      } else {
-        const float f = weights[row];
-        write_pair(c.seq, head0 + row, dim, o[i].x * f, o[i].y * f);
-        write_pair(c.seq, head0 + row, dim + 2, o[i].z * f, o[i].w * f);
-      }
-    }
-  };
-  // This warp has stored a piece of c's unit.  The last of the warps that do joins them, in the order of the
-  // list: the sum does not depend on who that is.
-  auto arrive = [&](const DenseCursor& c, const DensePieces& all) {
-    __threadfence();
-    __syncwarp();
-    uint32_t* counter = p.counters + int64_t(all.first) * p.side + member;
-    uint32_t seen = 0;
-    if (lane == 0) seen = atomicAdd(counter, 1u);
-    seen = __shfl_sync(0xffffffffu, seen, 0);
-    if (seen + 1 != uint32_t(all.count)) return;
-    __threadfence();
-    if (lane == 0) *counter = 0u;
-    join(std::false_type{}, c, all.count, [&](int i) {
-      const int r = dense_piece_run(cut, all, i);
-      return piece_of(r, dense_slot(cut, r, c.a));
-    }, nullptr);
   };
 
   // ---- stream ------------------------------------------------------------------------------------------
-  // (all teams of the CTA inside one unit group: they merge at the end)
-  bool merging = false;
-  if (teams > 1 && cut.begin(blockIdx.x * teams) < cut.total) {
-    DenseCursor c;
-    start(c, blockIdx.x * teams);
-    merging = dense_cta_merges(cut, blockIdx.x, c.a, c.b);
-  }
-#pragma unroll
-  for (int i = 0; i < S::kStages - 1; ++i) issue(i);
-  int stage = 0;
-  bool any_bad = false;
-  bool begun_before = false;  // the run's first unit has left a piece
-  DenseCursor before;
-  for (bool first = true; cu.at < cu.end; first = false) {
-    issue(stage == 0 ? S::kStages - 1 : stage - 1);
-    if (first || cu.at == cu.a) begin_unit();
+  int into = 0, from = 0;  // stages
+#pragma unroll 1
+  for (int step = 0;; ++step) {
+    if (waiting && made - used <= 16) store();
+    if (!waiting && !finished) describe();
+    issue(into);
+    into = into + 1 == S::kStages ? 0 : into + 1;
+    if (step < S::kStages - 1) continue;
+    if (used == made) break;
+    const int4 d = mine[used & 31];
+    if (d.z & 1 << 30) begin_unit(d);
     cp_async_wait<S::kStages - 1>();
     __syncwarp();
-    any_bad |= (bad >> stage) & 1;
-    tile_step(stage);
+    tile_step(from, d);
+    if (d.z < 0) flush(d);
     __syncwarp();
-    if (cu.at + 1 == cu.end) break;
-    if (cu.at + 1 == cu.b) {
-      if (cu.a >= cut.begin(run)) {
-        flush(nullptr);
-      } else {  // the join, if it falls to this warp, needs the ring: at the end
-        flush(piece_of(run, 0));
-        begun_before = true;
-        before = cu;
-      }
-    }
-    advance(cu);
-    stage = stage + 1 == S::kStages ? 0 : stage + 1;
+    ++used;
+    from = from + 1 == S::kStages ? 0 : from + 1;
   }
-  if (cut.begin(run) >= cut.end(run)) return;
-  if (any_bad && lane == 0) atomicOr(p.status, FQ_DEV_BAD_BLOCK_INDEX);
   cp_async_wait<0>();
-  __syncwarp();
-  const bool whole = cu.a >= cut.begin(run) && cu.b <= cut.end(run);
-  if (!merging) {
-    if (whole) flush(nullptr); else flush(piece_of(run, dense_slot(cut, run, cu.a)));
-    if (begun_before) arrive(before, dense_pieces(cut, before.a, before.b));
-    if (!whole) arrive(cu, dense_pieces(cut, cu.a, cu.b));
+}
+
+// A CTA per query head of a sequence and WIDE of its dimensions: weights of the pieces first, a thread to a piece,
+// then the sums.  A head whose unit one run had is left alone; one without tokens gets zeros.  What does not depend on
+// the pieces is done before the wait for the first kernel, and the first pieces are loaded with the weights.
+constexpr int kJoinThreads = 128;
+template <typename T, int D, int WIDE>
+__global__ void __launch_bounds__(kJoinThreads) dense_join_kernel(const DenseArgs p) {
+  constexpr int kLanes = WIDE / 4, kGroups = kJoinThreads / kLanes, kAhead = 4;
+  constexpr int kWarps = kJoinThreads / 32;
+  __shared__ float weights[kJoinThreads];
+  __shared__ float part[kWarps][2];
+  __shared__ int counts[kWarps][2];
+  __shared__ float4 sums[kGroups][kLanes];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int seq = blockIdx.x / p.hq, head = blockIdx.x - seq * p.hq;
+  const int heads = p.hq / p.hkv, kv = head / heads, in_group = head - kv * heads;
+  const int chunk = in_group / p.rows, row = in_group - chunk * p.rows;
+  const int unit = kv * p.chunks + chunk, group = unit / p.side, member = unit - group * p.side;
+  const int unit_groups = p.hkv * p.chunks / p.side;
+  const int column = tid % kLanes, mine = tid / kLanes;
+  const int64_t out_row = int64_t(seq) * p.hq + head;
+  T* const out = static_cast<T*>(p.out) + out_row * D + blockIdx.y * WIDE + 4 * column;
+  int s0, tiles, total;
+  if (p.seqs <= kJoinThreads) {
+    const int64_t room = int64_t(p.table_width) * p.block_size;
+    const int own = tid < p.seqs ? dense_span(p.lens[tid], room, p.window).tiles : 0;
+    int all = own, before = tid < seq ? own : 0;
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) {
+      all += __shfl_xor_sync(0xffffffffu, all, s);
+      before += __shfl_xor_sync(0xffffffffu, before, s);
+    }
+    if (lane == 0) {
+      counts[warp][0] = all;
+      counts[warp][1] = before;
+    }
+    __syncthreads();
+    total = s0 = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      total += counts[w][0] * unit_groups;
+      s0 += counts[w][1] * unit_groups;
+    }
+    tiles = dense_span(p.lens[seq], room, p.window).tiles;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+  } else {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    s0 = p.bounds[seq];
+    tiles = (p.bounds[seq + 1] - s0) / unit_groups;
+    total = p.bounds[p.seqs];
+  }
+  auto write = [&](float4 o) {
+    uint2 x;
+    x.x = Dense16<T>::pack(o.x, o.y);
+    x.y = Dense16<T>::pack(o.z, o.w);
+    *reinterpret_cast<uint2*>(out) = x;
+  };
+  if (tiles == 0) {
+    if (mine == 0) write(make_float4(0.f, 0.f, 0.f, 0.f));
+    if (p.lse && tid == 0 && blockIdx.y == 0) p.lse[out_row] = -INFINITY;
     return;
   }
-  flush(meet);
+  const DenseCut cut = dense_cut(total, p.fixed);
+  const int a = s0 + group * tiles;
+  const int first = cut.run_of(a), n = cut.run_of(a + tiles - 1) - first + 1;
+  if (n == 1) return;
+  // (only the first of its runs may hold it in slot 1)
+  const float* const pieces = p.pieces + (int64_t(first) * p.side + member) * 2 * p.piece_floats;
+  const int64_t stride = int64_t(p.side) * 2 * p.piece_floats;
+  const int64_t slot0 = dense_slot(cut, first, a) * p.piece_floats;
+  auto piece = [&](int i) { return pieces + i * stride + (i == 0 ? slot0 : 0); };
+  const int64_t offset = row * D + blockIdx.y * WIDE + 4 * column;
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float u, const float4& v) {
+    o.x = fmaf(u, v.x, o.x);
+    o.y = fmaf(u, v.y, o.y);
+    o.z = fmaf(u, v.z, o.z);
+    o.w = fmaf(u, v.w, o.w);
+  };
+  for (int i0 = 0; i0 < n; i0 += kJoinThreads) {
+    const int some = min(kJoinThreads, n - i0);
+    float2 x = make_float2(-INFINITY, 0.f);
+    if (tid < some) x = *reinterpret_cast<const float2*>(piece(i0 + tid) + p.rows * D + 2 * row);
+    float4 ahead[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = mine + k * kGroups;
+      if (i < some) ahead[k] = *reinterpret_cast<const float4*>(piece(i0 + i) + offset);
+    }
+    float now = x.x;
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, s));
+    __syncthreads();
+    if (lane == 0) part[warp][0] = now;
+    __syncthreads();
+    now = m;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) now = fmaxf(now, part[w][0]);
+    const float ref = now == -INFINITY ? 0.f : now;
+    const float w = fast_exp2(x.x - ref), f = fast_exp2(m - ref);
+    const float s = warp_sum(w * x.y);
+    weights[tid] = w;
+    if (lane == 0) part[warp][1] = s;
+    __syncthreads();
+    l *= f;
+#pragma unroll
+    for (int v = 0; v < kWarps; ++v) l += part[v][1];
+    m = now;
+    o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = mine + k * kGroups;
+      if (i < some) add(weights[i], ahead[k]);
+    }
+#pragma unroll 4
+    for (int i = mine + kAhead * kGroups; i < some; i += kGroups)
+      add(weights[i], *reinterpret_cast<const float4*>(piece(i0 + i) + offset));
+  }
+  if (mine < kGroups) sums[mine][column] = o;
   __syncthreads();
-  if (team > 0) return;
-  const DensePieces all = dense_pieces(cut, cu.a, cu.b);
-  float* dst = all.count == 1 ? nullptr : piece_of(run, dense_slot(cut, run, cu.a));
-  join(std::true_type{}, cu, teams, [&](int i) {
-    return reinterpret_cast<const float*>(smem + (i * p.side + warp) * S::kRing) + 33 * kRows;
-  }, dst);
-  if (dst) arrive(cu, all);
+  if (mine > 0) return;
+#pragma unroll
+  for (int i = 1; i < kGroups; ++i) add(1.f, sums[i][column]);
+  const float f = l == 0.f ? 0.f : 1.f / l;
+  write(make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+  if (p.lse && column == 0 && blockIdx.y == 0) p.lse[out_row] = dense_lse(m, l, Dense16<T>::kLift);
 }
 
 // ------------------------------------------------------------------------------------
@@ -585,8 +595,7 @@ static DenseGeometry dense_geometry(int hq, int hkv, int d) {
   x.r16 = group > 8;
   x.chunks = (group + 15) / 16;
   x.rows = (group + x.chunks - 1) / x.chunks;
-  const int warps = d > 128 ? 4 : 8;
-  x.side = warps;  // adjacent units to the warps of a CTA, as many as divide a sequence's units
+  x.side = dense_warps(d);  // adjacent units to the warps of a CTA, as many as divide a sequence's units
   while (hkv * x.chunks % x.side != 0) x.side /= 2;
   x.piece_floats = (x.rows * (d + 2) + 3) & ~3;
   return x;
@@ -614,6 +623,24 @@ static int dense_sms(int& sms) {
   return rc;
 }
 
+// A head's dimensions are split unless that makes many CTAs: one of a long sequence reads hundreds of pieces.
+constexpr int kJoinSplit = 8192;
+template <typename T, int D, int WIDE>
+static int launch_join(const DenseArgs& p, cudaStream_t stream) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(unsigned(p.seqs) * p.hq, D / WIDE);
+  config.blockDim = dim3(kJoinThreads);
+  config.stream = stream;
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&config, dense_join_kernel<T, D, WIDE>, p);
+  if (e != cudaSuccess) return fail(FQ_ERR_CUDA, "dense decode: %s", cudaGetErrorString(e));
+  return check_launch("dense decode, join");
+}
+
 template <typename T, int D, bool R16>
 static int launch_dense(const DenseArgs& p, int ctas, cudaStream_t stream) {
   using S = DenseShape<D>;
@@ -631,7 +658,9 @@ static int launch_dense(const DenseArgs& p, int ctas, cudaStream_t stream) {
     }
   }
   kernel<<<ctas, S::kWarps * 32, smem, stream>>>(p);
-  return check_launch("dense decode");
+  if (const int rc = check_launch("dense decode")) return rc;
+  return int64_t(p.seqs) * p.hq * (D / 32) > kJoinSplit ? launch_join<T, D, D>(p, stream)
+                                                        : launch_join<T, D, 32>(p, stream);
 }
 template <typename T, int D>
 static int launch_dense(const DenseArgs& p, bool r16, int ctas, cudaStream_t stream) {
@@ -660,8 +689,8 @@ extern "C" size_t fq_dense_paged_decode_workspace_bytes(int num_seqs, int num_q_
                                                         int head_dim) {
   if (!dense_shape_ok(num_seqs, num_q_heads, num_kv_heads, head_dim)) return 0;
   const DenseGeometry x = dense_geometry(num_q_heads, num_kv_heads, head_dim);
-  const size_t warps = head_dim > 128 ? 4 : 8;
-  return kDenseHead + kDenseMaxCtas * warps * 2 * size_t(x.piece_floats) * sizeof(float);
+  const size_t warps = dense_warps(head_dim);
+  return kDensePieces + kDenseMaxCtas * warps * (1 + kDenseTaken) * 2 * size_t(x.piece_floats) * sizeof(float);
 }
 
 extern "C" int fq_dense_paged_decode(
@@ -680,8 +709,8 @@ extern "C" int fq_dense_paged_decode(
   FQ_REQUIRE(dense_shape_ok(num_seqs, num_q_heads, num_kv_heads, head_dim), FQ_ERR_UNSUPPORTED,
              "dense decode: head_dim 64, 96, 128 or 256, at most %d sequences and 1024 query heads (got %d, %d, %d)",
              kDenseMaxSeqs, head_dim, num_seqs, num_q_heads);
-  FQ_REQUIRE(block_size > 0 && block_size % kDenseTile == 0, FQ_ERR_UNSUPPORTED,
-             "dense decode: block_size must be a multiple of %d (got %d)", kDenseTile, block_size);
+  FQ_REQUIRE(block_size > 0 && block_size % kDenseTile == 0 && block_size <= kDenseMaxBlock, FQ_ERR_UNSUPPORTED,
+             "dense decode: block_size must be a multiple of %d, at most 2^22 (got %d)", kDenseTile, block_size);
   if (num_seqs == 0) return FQ_OK;
   FQ_REQUIRE(q && seq_lens && out, FQ_ERR_INVALID_ARGUMENT, "dense decode: null pointer");
   FQ_REQUIRE(block_table_width == 0 || (block_table && key_cache && value_cache), FQ_ERR_INVALID_ARGUMENT,
@@ -711,15 +740,16 @@ extern "C" int fq_dense_paged_decode(
   p.scale_log2 = sm_scale * 1.44269504f;
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   p.status = reinterpret_cast<uint32_t*>(ws);
-  p.counters = reinterpret_cast<uint32_t*>(ws + kDenseCounters);
-  p.pieces = reinterpret_cast<float*>(ws + kDenseHead);
-  // one CTA per SM (the rings fill its shared memory); no more than there can be runs, or rows without a token
-  const int teams = (head_dim > 128 ? 4 : 8) / x.side;
-  const int64_t runs = (most + kDenseShortest - 1) / kDenseShortest;
-  const int64_t want = (runs + teams - 1) / teams;
+  p.tickets = reinterpret_cast<uint32_t*>(ws + kDenseTickets);
+  p.bounds = reinterpret_cast<int*>(ws + kDenseBounds);
+  p.pieces = reinterpret_cast<float*>(ws + kDensePieces);
+  // one CTA per SM (the rings fill its shared memory), no more than there can be runs
   int sms = 0;
   if (const int rc = dense_sms(sms)) return rc;
-  const int ctas = int(std::min<int64_t>(sms, std::max<int64_t>(want, std::min(num_seqs, 16))));
+  const int teams = dense_warps(head_dim) / x.side;
+  const int64_t runs = (most + kDenseShortest - 1) / kDenseShortest;
+  const int ctas = int(std::max<int64_t>(1, std::min<int64_t>(sms, (runs + teams - 1) / teams)));
+  p.fixed = ctas * teams;
   return dtype == FQ_F16 ? launch_dense<__half>(p, head_dim, x.r16, ctas, stream)
                          : launch_dense<__nv_bfloat16>(p, head_dim, x.r16, ctas, stream);
 }

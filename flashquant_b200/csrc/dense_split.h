@@ -1,11 +1,15 @@
 // How the one-token attention over 16-bit pages is cut into runs, and what each run owes to the others.
-// Plain integer arithmetic, the same on the host (where it is tested) and in the kernel.
+// Plain integer arithmetic, the same on the host (where it is tested) and in the kernels.
 //
 // A "unit" is what one warp attends with: up to 16 query heads of one KV head of one sequence.  `side` units
-// of a sequence stand side by side in a CTA (adjacent warps read adjacent heads of the same tokens, so the
-// rows of a page are read whole); the CTA has `teams` = warps / side such rows of warps.  The tiles of 16
-// tokens of all unit groups of all sequences form one list of `total` entries, cut into runs of `length`, run
-// i for team i % teams of CTA i / teams.  Ragged batches are balanced whatever their lengths.
+// of a sequence stand side by side (they are given to warps that run at the same time, so that the heads of a
+// token, which are adjacent in a page, are read together).  The tiles of 16 tokens of all unit groups of all
+// sequences form one list of `total` entries, cut into runs whatever the bounds between sequences are: a ragged
+// batch is balanced.  Where a warp's share is long enough, thirteen sixteenths of the list
+// are dealt out beforehand and the rest in runs of a sixteenth, then a thirty-second, of a share that warps take
+// when they are free: SMs do not get
+// the same share of the memory's bandwidth (8 sequences of 32k - 131k tokens, equal runs: the first SM was
+// through after 345 us, the last after 483).  Where the cuts are never depends on who takes a run.
 #pragma once
 
 #include <stdint.h>
@@ -38,56 +42,52 @@ FQ_HD DenseSpan dense_span(int len, int64_t room, int window) {
 }
 
 struct DenseCut {
-  int total;   // entries of the list
-  int length;  // of a run
-  int teams;   // runs of a CTA
-  FQ_HD int run_of(int at) const { return at / length; }
+  int total;             // entries of the list
+  int fixed;             // runs that are dealt out beforehand
+  int length, bound;     // of such a run; fixed * length, or total if that is all
+  int medium, length2;   // runs behind `bound`, then
+  int bound2, length3;   // runs behind bound2 to the end
+  FQ_HD int run_of(int at) const {
+    return at < bound ? at / length
+                      : (at < bound2 ? fixed + (at - bound) / length2 : fixed + medium + (at - bound2) / length3);
+  }
   FQ_HD int begin(int run) const {
-    const int64_t x = int64_t(run) * length;
+    const int64_t x = run < fixed ? int64_t(run) * length
+                                  : (run < fixed + medium ? bound + int64_t(run - fixed) * length2
+                                                          : bound2 + int64_t(run - fixed - medium) * length3);
     return x < total ? int(x) : total;
   }
   FQ_HD int end(int run) const { return begin(run + 1); }
+  FQ_HD int taken() const { return medium + (total - bound2 + length3 - 1) / length3; }
 };
-// At least `shortest` tiles to a run (a short list is not cut finer: its parts have to be joined again).
-FQ_HD DenseCut dense_cut(int total, int ctas, int teams, int shortest) {
-  const int64_t runs = int64_t(ctas) * teams;
-  int length = int((total + runs - 1) / runs);
-  if (length < shortest) length = shortest;
-  return DenseCut{total, length, teams};
+constexpr int kDenseShare = 32;   // tiles of a share from which on a part of the list is taken
+constexpr int kDenseTaken = 6;    // runs taken per share, at most
+constexpr int kDenseShortest = 2; // tiles of a run at least, where there are enough
+FQ_HD DenseCut dense_cut(int total, int fixed) {
+  DenseCut c;
+  const int share = int((int64_t(total) + fixed - 1) / fixed);
+  c.total = total;
+  c.fixed = fixed;
+  c.length = share < kDenseShortest ? kDenseShortest : share;
+  c.bound = c.bound2 = total;
+  c.medium = 0;
+  c.length2 = c.length3 = 1;
+  if (share < kDenseShare) return c;
+  c.length2 = (share + 15) / 16;
+  c.length3 = (share + 31) / 32;
+  c.length = share - 3 * c.length2;
+  const int64_t bound = int64_t(c.length) * fixed;
+  if (bound >= total) return c;
+  c.bound = int(bound);
+  const int64_t medium = int64_t(fixed) * 2, fits = (total - c.bound) / c.length2;
+  c.medium = int(medium < fits ? medium : fits);
+  c.bound2 = c.bound + c.medium * c.length2;
+  return c;
 }
 
 // A unit group takes the entries [a, b) of the list.  A run that holds all of them writes its result; the
-// others leave a piece.  A run has at most two pieces: the one that was begun before it (slot 0) and the one
-// that goes on behind it (slot 1).
+// others leave a piece.  A run has at most two pieces: of the group that was begun before it (slot 0) and of the
+// one that goes on behind it (slot 1).  The pieces of a group are those of its runs, run_of(a) to run_of(b - 1).
 FQ_HD int dense_slot(const DenseCut& c, int run, int a) { return a < c.begin(run) ? 0 : 1; }
-// The teams of a CTA that are all inside one unit group merge first and leave one piece.
-FQ_HD bool dense_cta_merges(const DenseCut& c, int cta, int a, int b) {
-  const int first = cta * c.teams, last = first + c.teams - 1;
-  return c.begin(first) >= a && c.begin(last) < b && c.end(last) <= b;
-}
-// The pieces of a unit group, in the order of the list: `before` runs, `whole` merging CTAs that count once
-// each, then runs again.
-struct DensePieces {
-  int first, before, cta, whole, count;
-};
-FQ_HD DensePieces dense_pieces(const DenseCut& c, int a, int b) {
-  DensePieces p;
-  const int last = c.run_of(b - 1);
-  p.first = c.run_of(a);
-  const int inner = (a + c.length - 1) / c.length;                 // the first run that begins inside
-  const int after = b == c.total ? last + 1 : b / c.length;        // behind the last one that ends inside
-  p.cta = (inner + c.teams - 1) / c.teams;
-  p.whole = after / c.teams - p.cta;
-  if (c.teams == 1 || p.whole < 0) p.whole = 0;
-  p.before = p.whole ? p.cta * c.teams - p.first : 0;
-  p.count = last - p.first + 1 - p.whole * (c.teams - 1);
-  return p;
-}
-// the run whose slots hold piece i (of a merging CTA: its first)
-FQ_HD int dense_piece_run(const DenseCut& c, const DensePieces& p, int i) {
-  if (p.whole == 0 || i < p.before) return p.first + i;
-  if (i < p.before + p.whole) return (p.cta + i - p.before) * c.teams;
-  return (p.cta + p.whole) * c.teams + i - p.before - p.whole;
-}
 
 }  // namespace fq

@@ -14,53 +14,61 @@ from flashquant_b200 import _native as N
 from flashquant_b200 import dense
 from conftest import ROOT
 
-# Walks every run of a list as a warp does and checks what the arithmetic says of it: every tile in one run, every
-# unit group joined from exactly the pieces that its runs leave, in order, each in a slot of its own.
+# Every tile in one run, every piece of a unit group in a slot of its own, as many runs as the workspace has room for.
 _DRIVER = r"""
 #include <cstdio>
 #include <cstdlib>
-#include <map>
 #include <set>
 #include <utility>
 #include <vector>
 #include "dense_split.h"
 using namespace fq;
-#define CHECK(x) do { if (!(x)) { std::printf("%s: total %d teams %d ctas %d unit [%d, %d)\n", #x, c.total, c.teams, ctas, a, b); return 1; } } while (0)
+#define CHECK(x) do { if (!(x)) { std::printf("%s: total %d fixed %d unit [%d, %d)\n", #x, c.total, c.fixed, a, b); return 1; } } while (0)
 int main() {
   std::srand(7);
   for (int round = 0; round < 20000; ++round) {
-    const int teams = 1 << std::rand() % 4, ctas = 1 + std::rand() % (round % 2 ? 148 : 9);
+    const int fixed = 1 + std::rand() % (round % 2 ? 1184 : 9);
     std::vector<int> bound{0};
-    const int units = 1 + std::rand() % 40, longest = 1 + std::rand() % (round % 3 ? 30 : 3000);
+    const int units = 1 + std::rand() % 40, longest = 1 + std::rand() % (round % 3 ? 30 : 30000);
     for (int i = 0; i < units; ++i) bound.push_back(bound.back() + 1 + std::rand() % longest);
-    const DenseCut c = dense_cut(bound.back(), ctas, teams, 1 + std::rand() % 5);
+    const DenseCut c = dense_cut(bound.back(), fixed);
+    const int runs = c.fixed + c.taken();
     int a = 0, b = 0;
-    CHECK(c.end(ctas * teams - 1) == c.total && c.begin(0) == 0);
-    for (int r = 1; r < ctas * teams; ++r) CHECK(c.begin(r) == c.end(r - 1));
+    CHECK(c.begin(0) == 0 && c.end(runs - 1) == c.total && c.taken() <= kDenseTaken * fixed);
+    for (int r = 1; r < runs; ++r) CHECK(c.begin(r) == c.end(r - 1) && c.begin(r) <= c.end(r));
+    for (int r = c.fixed; r < runs; ++r) CHECK(c.begin(r) < c.end(r));
+    for (int i = 0; i < 20; ++i) {
+      const int at = std::rand() % c.total, r = c.run_of(at);
+      CHECK(r >= 0 && r < runs && c.begin(r) <= at && at < c.end(r));
+    }
+    if (c.taken()) CHECK(c.end(c.fixed - 1) == c.fixed * c.length);
     std::set<std::pair<int, int>> slots;
-    std::set<int> counters;
     for (int u = 0; u < units; ++u) {
       a = bound[u], b = bound[u + 1];
-      const DensePieces p = dense_pieces(c, a, b);
       if (c.run_of(a) == c.run_of(b - 1)) continue;  // one run has it
-      CHECK(counters.insert(p.first).second && p.first < ctas * teams);
-      std::vector<int> from;  // runs that leave a piece
-      for (int r = 0; r < ctas * teams; ++r) {
-        if (c.end(r) <= a || c.begin(r) >= b) continue;
-        if (dense_cta_merges(c, r / teams, a, b) && r % teams && teams > 1) continue;
-        from.push_back(r);
+      for (int r = c.run_of(a); r <= c.run_of(b - 1); ++r) {
+        CHECK(c.begin(r) < b && c.end(r) > a && c.begin(r) < c.end(r));
         CHECK(slots.insert({r, dense_slot(c, r, a)}).second);
       }
-      CHECK(int(from.size()) == p.count);
-      for (int i = 0; i < p.count; ++i) CHECK(dense_piece_run(c, p, i) == from[i]);
     }
+  }
+  for (int total : {1, 31 * 1184, 32 * 1184, 1 << 30, (1 << 30) - 1}) {
+    const DenseCut c = dense_cut(total, 1184);
+    int a = 0, b = total;
+    CHECK(c.end(c.fixed + c.taken() - 1) == total && c.run_of(total - 1) < c.fixed + (c.taken() ? c.taken() : 1));
+    CHECK(c.taken() <= kDenseTaken * 1184);
+  }
+  {
+    const DenseCut c = dense_cut(0, 148);
+    int a = 0, b = 0;
+    CHECK(c.taken() == 0 && c.begin(0) == 0 && c.end(147) == 0);
   }
   for (int len = -3; len < 200; ++len)
     for (int window = 0; window < 70; ++window)
       for (int room = 0; room <= 160; room += 16) {
         const DenseSpan s = dense_span(len, room, window);
-        const DenseCut c{len, window, room};
-        int a = s.begin, b = s.len, ctas = s.tiles;
+        const DenseCut c = dense_cut(len < 0 ? 0 : len, 1 + window);
+        int a = s.begin, b = s.len;
         CHECK(b >= 0 && b <= room && (len < 0 || b <= len) && a >= 0 && a <= b && s.tiles >= 0);
         CHECK(b == 0 || (b - a == (window && window < b ? window : b)));
         CHECK(16 * s.first_tile <= a && a - 16 * s.first_tile < 16 && 16 * (s.first_tile + s.tiles) >= b);
