@@ -44,6 +44,7 @@ struct DenseArgs {
   int side, piece_floats;                // units side by side; stride of the pieces
   float scale_log2;
   int fixed;                             // runs dealt out beforehand
+  int join_rows, join_wide;              // heads and dimensions of a CTA of the join
   uint32_t *status, *tickets;
   int* bounds;
   float* pieces;                         // [run][side][slot]: [rows][D], [rows][2] (maximum, sum)
@@ -67,8 +68,11 @@ struct DenseShape {
   static __device__ __forceinline__ int key(int row) { return D == 96 ? row >> 1 & 3 : row & 7; }
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0)
+// (keys and values are read once: with a hint that keeps the L2 for what is used again, the pieces, the tables and
+// the kernels' code among it)
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src),
+               "r"(valid ? 16 : 0), "l"(policy)
                : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -252,6 +256,7 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
   };
 
   const uint32_t ring = smem_u32(smem) + warp * S::kRing;
+  const uint64_t policy = l2_evict_first_policy();
   constexpr int kPerRow = D / 8, kChunks = kDenseTile * kPerRow / 32;
   // one tile on its way, if there is one (each call is a group: tile n is complete when group n is)
   auto issue = [&](int stage) {
@@ -274,8 +279,8 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
         const int i = lane + 32 * c, r = i / kPerRow, col = i % kPerRow;
         const bool valid = r >= lo && r < hi;
         const uint32_t to = dst + r * S::kRow + ((col ^ S::key(r)) << 4);
-        cp_async16(to, k + (valid ? r * p.k_token + col * 8 : 0), valid);
-        cp_async16(to + S::kTensor, v + (valid ? r * p.v_token + col * 8 : 0), valid);
+        cp_async16(to, k + (valid ? r * p.k_token + col * 8 : 0), valid, policy);
+        cp_async16(to + S::kTensor, v + (valid ? r * p.v_token + col * 8 : 0), valid, policy);
       }
     }
     cp_async_commit();
@@ -453,31 +458,37 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
   cp_async_wait<0>();
 }
 
-// A CTA per query head of a sequence and WIDE of its dimensions: weights of the pieces first, a thread to a piece,
-// then the sums.  A head whose unit one run had is left alone; one without tokens gets zeros.  What does not depend on
-// the pieces is done before the wait for the first kernel, and the first pieces are loaded with the weights.
-constexpr int kJoinThreads = 128;
-template <typename T, int D, int WIDE>
-__global__ void __launch_bounds__(kJoinThreads) dense_join_kernel(const DenseArgs p) {
-  constexpr int kLanes = WIDE / 4, kGroups = kJoinThreads / kLanes, kAhead = 4;
-  constexpr int kWarps = kJoinThreads / 32;
-  __shared__ float weights[kJoinThreads];
-  __shared__ float part[kWarps][2];
+// A CTA for `join_rows` query heads of a unit and `join_wide` of their dimensions: the weights of the pieces first, a warp
+// to a head and a lane to a piece, then the sums, a group of threads to a piece.  A unit that one run had is left alone;
+// heads without tokens get zeros.  What does not depend on the pieces is done before the wait for the first kernel, and
+// the first pieces are on their way with the weights.
+constexpr int kJoinThreads = 256, kJoinPieces = 128, kJoinRows = 8;
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads, 4) dense_join_kernel(const DenseArgs p) {
+  constexpr int kAhead = 6, kWarps = kJoinThreads / 32;
+  __shared__ float weights[kJoinRows][kJoinPieces];
+  __shared__ float totals[kJoinRows][3];  // maximum, sum, factor of what stands
   __shared__ int counts[kWarps][2];
-  __shared__ float4 sums[kGroups][kLanes];
+  __shared__ float4 sums[kJoinThreads];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int seq = blockIdx.x / p.hq, head = blockIdx.x - seq * p.hq;
-  const int heads = p.hq / p.hkv, kv = head / heads, in_group = head - kv * heads;
-  const int chunk = in_group / p.rows, row = in_group - chunk * p.rows;
-  const int unit = kv * p.chunks + chunk, group = unit / p.side, member = unit - group * p.side;
-  const int unit_groups = p.hkv * p.chunks / p.side;
-  const int column = tid % kLanes, mine = tid / kLanes;
-  const int64_t out_row = int64_t(seq) * p.hq + head;
-  T* const out = static_cast<T*>(p.out) + out_row * D + blockIdx.y * WIDE + 4 * column;
+  const int units = p.hkv * p.chunks, unit_groups = units / p.side;
+  const int seq = blockIdx.x / units, unit = blockIdx.x - seq * units;
+  const int group = unit / p.side, member = unit - group * p.side;
+  const DenseUnit u = dense_unit(p, unit);
+  const int wides = D / p.join_wide, row0 = blockIdx.y / wides * p.join_rows;
+  const int rows = min(p.join_rows, u.count - row0);
+  if (rows <= 0) return;
+  const int columns = p.join_rows * p.join_wide / 4, groups = kJoinThreads / columns;  // float4
+  const int mine = tid / columns, column = tid - mine * columns;
+  const int row = column * 4 / p.join_wide;
+  const int dim = (blockIdx.y % wides) * p.join_wide + column * 4 - row * p.join_wide;
+  const bool real = row < rows && mine < groups;
+  const int64_t out_row = int64_t(seq) * p.hq + u.head0 + row0;
   int s0, tiles, total;
   if (p.seqs <= kJoinThreads) {
     const int64_t room = int64_t(p.table_width) * p.block_size;
     const int own = tid < p.seqs ? dense_span(p.lens[tid], room, p.window).tiles : 0;
+    tiles = dense_span(p.lens[seq], room, p.window).tiles;
     int all = own, before = tid < seq ? own : 0;
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) {
@@ -495,8 +506,6 @@ __global__ void __launch_bounds__(kJoinThreads) dense_join_kernel(const DenseArg
       total += counts[w][0] * unit_groups;
       s0 += counts[w][1] * unit_groups;
     }
-    tiles = dense_span(p.lens[seq], room, p.window).tiles;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
   } else {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     s0 = p.bounds[seq];
@@ -507,11 +516,12 @@ __global__ void __launch_bounds__(kJoinThreads) dense_join_kernel(const DenseArg
     uint2 x;
     x.x = Dense16<T>::pack(o.x, o.y);
     x.y = Dense16<T>::pack(o.z, o.w);
-    *reinterpret_cast<uint2*>(out) = x;
+    *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (out_row + row) * D + dim) = x;
   };
+  const bool with_lse = p.lse && blockIdx.y % wides == 0;
   if (tiles == 0) {
-    if (mine == 0) write(make_float4(0.f, 0.f, 0.f, 0.f));
-    if (p.lse && tid == 0 && blockIdx.y == 0) p.lse[out_row] = -INFINITY;
+    if (real && mine == 0) write(make_float4(0.f, 0.f, 0.f, 0.f));
+    if (with_lse && tid < rows) p.lse[out_row + tid] = -INFINITY;
     return;
   }
   const DenseCut cut = dense_cut(total, p.fixed);
@@ -523,62 +533,74 @@ __global__ void __launch_bounds__(kJoinThreads) dense_join_kernel(const DenseArg
   const int64_t stride = int64_t(p.side) * 2 * p.piece_floats;
   const int64_t slot0 = dense_slot(cut, first, a) * p.piece_floats;
   auto piece = [&](int i) { return pieces + i * stride + (i == 0 ? slot0 : 0); };
-  const int64_t offset = row * D + blockIdx.y * WIDE + 4 * column;
-  float m = -INFINITY, l = 0.f;
+  const int64_t offset = (row0 + row) * D + dim;
+  float m = -INFINITY, l = 0.f;  // of row `warp`
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](float u, const float4& v) {
-    o.x = fmaf(u, v.x, o.x);
-    o.y = fmaf(u, v.y, o.y);
-    o.z = fmaf(u, v.z, o.z);
-    o.w = fmaf(u, v.w, o.w);
+  auto add = [&](float w, const float4& v) {
+    o.x = fmaf(w, v.x, o.x);
+    o.y = fmaf(w, v.y, o.y);
+    o.z = fmaf(w, v.z, o.z);
+    o.w = fmaf(w, v.w, o.w);
   };
-  for (int i0 = 0; i0 < n; i0 += kJoinThreads) {
-    const int some = min(kJoinThreads, n - i0);
-    float2 x = make_float2(-INFINITY, 0.f);
-    if (tid < some) x = *reinterpret_cast<const float2*>(piece(i0 + tid) + p.rows * D + 2 * row);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int i0 = 0; i0 < n; i0 += kJoinPieces) {
+    const int some = min(kJoinPieces, n - i0);
     float4 ahead[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      const int i = mine + k * kGroups;
-      if (i < some) ahead[k] = *reinterpret_cast<const float4*>(piece(i0 + i) + offset);
+      const int i = mine + k * groups;
+      if (real && i < some) ahead[k] = *reinterpret_cast<const float4*>(piece(i0 + i) + offset);
     }
-    float now = x.x;
+    if (i0) __syncthreads();  // the weights before have been used
+    if (warp < rows) {
+      float2 x[kJoinPieces / 32];
+      float now = m;
 #pragma unroll
-    for (int s = 16; s > 0; s >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, s));
-    __syncthreads();
-    if (lane == 0) part[warp][0] = now;
-    __syncthreads();
-    now = m;
+      for (int k = 0; k < kJoinPieces / 32; ++k) {
+        const int i = lane + 32 * k;
+        x[k] = make_float2(-INFINITY, 0.f);
+        if (i < some) x[k] = *reinterpret_cast<const float2*>(piece(i0 + i) + p.rows * D + 2 * (row0 + warp));
+      }
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) now = fmaxf(now, part[w][0]);
-    const float ref = now == -INFINITY ? 0.f : now;
-    const float w = fast_exp2(x.x - ref), f = fast_exp2(m - ref);
-    const float s = warp_sum(w * x.y);
-    weights[tid] = w;
-    if (lane == 0) part[warp][1] = s;
-    __syncthreads();
-    l *= f;
+      for (int k = 0; k < kJoinPieces / 32; ++k) now = fmaxf(now, x[k].x);
 #pragma unroll
-    for (int v = 0; v < kWarps; ++v) l += part[v][1];
-    m = now;
+      for (int s = 16; s > 0; s >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, s));
+      const float ref = now == -INFINITY ? 0.f : now, f = fast_exp2(m - ref);
+      float s = 0.f;
+#pragma unroll
+      for (int k = 0; k < kJoinPieces / 32; ++k) {
+        const float w = fast_exp2(x[k].x - ref);
+        s = fmaf(w, x[k].y, s);
+        weights[warp][lane + 32 * k] = w;
+      }
+      l = fmaf(l, f, warp_sum(s));
+      m = now;
+      if (lane == 0) {
+        totals[warp][0] = m;
+        totals[warp][1] = l;
+        totals[warp][2] = f;
+      }
+    }
+    __syncthreads();
+    if (!real) continue;
+    const float f = totals[row][2];
     o.x *= f; o.y *= f; o.z *= f; o.w *= f;
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      const int i = mine + k * kGroups;
-      if (i < some) add(weights[i], ahead[k]);
+      const int i = mine + k * groups;
+      if (i < some) add(weights[row][i], ahead[k]);
     }
-#pragma unroll 4
-    for (int i = mine + kAhead * kGroups; i < some; i += kGroups)
-      add(weights[i], *reinterpret_cast<const float4*>(piece(i0 + i) + offset));
+#pragma unroll 6
+    for (int i = mine + kAhead * groups; i < some; i += groups)
+      add(weights[row][i], *reinterpret_cast<const float4*>(piece(i0 + i) + offset));
   }
-  if (mine < kGroups) sums[mine][column] = o;
+  sums[tid] = o;
   __syncthreads();
-  if (mine > 0) return;
-#pragma unroll
-  for (int i = 1; i < kGroups; ++i) add(1.f, sums[i][column]);
-  const float f = l == 0.f ? 0.f : 1.f / l;
+  if (with_lse && tid < rows) p.lse[out_row + tid] = dense_lse(totals[tid][0], totals[tid][1], Dense16<T>::kLift);
+  if (!real || mine > 0) return;
+  for (int i = 1; i < groups; ++i) add(1.f, sums[i * columns + column]);
+  const float all = totals[row][1], f = all == 0.f ? 0.f : 1.f / all;
   write(make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
-  if (p.lse && column == 0 && blockIdx.y == 0) p.lse[out_row] = dense_lse(m, l, Dense16<T>::kLift);
 }
 
 // ------------------------------------------------------------------------------------
@@ -623,12 +645,18 @@ static int dense_sms(int& sms) {
   return rc;
 }
 
-// A head's dimensions are split unless that makes many CTAs: one of a long sequence reads hundreds of pieces.
-constexpr int kJoinSplit = 8192;
-template <typename T, int D, int WIDE>
-static int launch_join(const DenseArgs& p, cudaStream_t stream) {
+// As many heads to a CTA of the join as leave it with less than four CTAs on an SM, all resident at once; where there are
+// few heads, their dimensions are split.  (32 sequences, 32 heads: a CTA per head and 32 dimensions 17 us, ...)
+template <typename T, int D>
+static int launch_join(DenseArgs p, cudaStream_t stream) {
+  const int64_t units = int64_t(p.seqs) * p.hkv * p.chunks;
+  p.join_rows = 1;
+  p.join_wide = units * p.rows * (D / 32) <= 4 * kDenseMaxCtas ? 32 : D;
+  while (p.join_rows < p.rows && 2 * p.join_rows <= kJoinRows && 2 * p.join_rows * p.join_wide / 4 <= kJoinThreads &&
+         units * ((p.rows + p.join_rows - 1) / p.join_rows) * (D / p.join_wide) > 4 * kDenseMaxCtas)
+    p.join_rows *= 2;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(unsigned(p.seqs) * p.hq, D / WIDE);
+  config.gridDim = dim3(unsigned(units), (p.rows + p.join_rows - 1) / p.join_rows * (D / p.join_wide));
   config.blockDim = dim3(kJoinThreads);
   config.stream = stream;
   cudaLaunchAttribute early;
@@ -636,7 +664,7 @@ static int launch_join(const DenseArgs& p, cudaStream_t stream) {
   early.val.programmaticStreamSerializationAllowed = 1;
   config.attrs = &early;
   config.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&config, dense_join_kernel<T, D, WIDE>, p);
+  const cudaError_t e = cudaLaunchKernelEx(&config, dense_join_kernel<T, D>, p);
   if (e != cudaSuccess) return fail(FQ_ERR_CUDA, "dense decode: %s", cudaGetErrorString(e));
   return check_launch("dense decode, join");
 }
@@ -659,8 +687,7 @@ static int launch_dense(const DenseArgs& p, int ctas, cudaStream_t stream) {
   }
   kernel<<<ctas, S::kWarps * 32, smem, stream>>>(p);
   if (const int rc = check_launch("dense decode")) return rc;
-  return int64_t(p.seqs) * p.hq * (D / 32) > kJoinSplit ? launch_join<T, D, D>(p, stream)
-                                                        : launch_join<T, D, 32>(p, stream);
+  return launch_join<T, D>(p, stream);
 }
 template <typename T, int D>
 static int launch_dense(const DenseArgs& p, bool r16, int ctas, cudaStream_t stream) {

@@ -65,7 +65,7 @@ constexpr int kDenseTaken = 6;    // runs taken per share, at most
 constexpr int kDenseShortest = 2; // tiles of a run at least, where there are enough
 FQ_HD DenseCut dense_cut(int total, int fixed) {
   DenseCut c;
-  const int share = int((int64_t(total) + fixed - 1) / fixed);
+  const int share = (total + fixed - 1) / fixed;  // (total below 2^30)
   c.total = total;
   c.fixed = fixed;
   c.length = share < kDenseShortest ? kDenseShortest : share;
@@ -79,8 +79,8 @@ FQ_HD DenseCut dense_cut(int total, int fixed) {
   const int64_t bound = int64_t(c.length) * fixed;
   if (bound >= total) return c;
   c.bound = int(bound);
-  const int64_t medium = int64_t(fixed) * 2, fits = (total - c.bound) / c.length2;
-  c.medium = int(medium < fits ? medium : fits);
+  const int fits = (total - c.bound) / c.length2;
+  c.medium = fits < 2 * fixed ? fits : 2 * fixed;
   c.bound2 = c.bound + c.medium * c.length2;
   return c;
 }
