@@ -47,7 +47,7 @@ struct DenseArgs {
   int join_rows, join_wide;              // heads and dimensions of a CTA of the join
   uint32_t *status, *tickets;
   int* bounds;
-  float* pieces;                         // [run][side][slot]: [rows][D], [rows][2] (maximum, sum)
+  float* pieces;                         // [slot][side]: [rows][D], [rows][2] (maximum, sum)
 };
 
 // Warps of a CTA, one CTA per SM: as many as the registers leave (a row of the accumulators is D floats).  head_dim 64,
@@ -221,14 +221,15 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
     }
     waiting = min(16, end - at);
     if (lane < waiting) {
-      const int here = at + lane;
+      const bool tail = cut.is_tail(run);
+      const int i = at + lane, here = cut.entry(tail, i);
       int lo = 0, hi = p.seqs - 1;  // the sequence whose entries hold `here`
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
         if (prefix[mid + 1] > here) hi = mid; else lo = mid + 1;
       }
       const DenseSpan span = dense_span(lengths[lo], room, p.window);
-      const int group = (here - prefix[lo]) / span.tiles;
+      const int group = unit_groups == 1 ? 0 : (here - prefix[lo]) / span.tiles;
       const int a = prefix[lo] + group * span.tiles, b = a + span.tiles;
       const int tile = span.first_tile + here - a;
       const int page = tile / tiles_per_block, first = tile * kDenseTile;
@@ -236,9 +237,10 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
       next.y = (tile - page * tiles_per_block) * kDenseTile | max(span.begin - first, 0) << 22 |
                min(span.len - first, kDenseTile) << 26;
       next.z = lo | (group * p.side + member) << 12;
-      if (here == a || here == cut.begin(run)) next.z |= 1 << 30;
-      if (here + 1 == b || here + 1 == end) next.z |= 1 << 31;
-      next.w = a >= cut.begin(run) && b <= end ? -1 : (run * p.side + member) * 2 + dense_slot(cut, run, a);
+      if (i == cut.kind_of(tail, a) || i == cut.begin(run)) next.z |= 1 << 30;
+      if (i + 1 == cut.kind_of(tail, b) || i + 1 == end) next.z |= 1 << 31;
+      const int nth = lo * unit_groups + group;
+      next.w = dense_whole(cut, run, a, b) ? -1 : dense_slot(cut, run, nth, p.seqs * unit_groups) * p.side + member;
     }
     at += waiting;
   };
@@ -462,10 +464,10 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
 // to a head and a lane to a piece, then the sums, a group of threads to a piece.  A unit that one run had is left alone;
 // heads without tokens get zeros.  What does not depend on the pieces is done before the wait for the first kernel, and
 // the first pieces are on their way with the weights.
-constexpr int kJoinThreads = 256, kJoinPieces = 128, kJoinRows = 8;
+constexpr int kJoinThreads = 128, kJoinPieces = 128, kJoinRows = 4;
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoinThreads, 4) dense_join_kernel(const DenseArgs p) {
-  constexpr int kAhead = 6, kWarps = kJoinThreads / 32;
+__global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const DenseArgs p) {
+  constexpr int kAhead = 4, kWarps = kJoinThreads / 32;
   __shared__ float weights[kJoinRows][kJoinPieces];
   __shared__ float totals[kJoinRows][3];  // maximum, sum, factor of what stands
   __shared__ int counts[kWarps][2];
@@ -526,13 +528,13 @@ __global__ void __launch_bounds__(kJoinThreads, 4) dense_join_kernel(const Dense
   }
   const DenseCut cut = dense_cut(total, p.fixed);
   const int a = s0 + group * tiles;
-  const int first = cut.run_of(a), n = cut.run_of(a + tiles - 1) - first + 1;
+  const DensePieces all = dense_pieces(cut, a, a + tiles);
+  const int n = all.count();
   if (n == 1) return;
-  // (only the first of its runs may hold it in slot 1)
-  const float* const pieces = p.pieces + (int64_t(first) * p.side + member) * 2 * p.piece_floats;
-  const int64_t stride = int64_t(p.side) * 2 * p.piece_floats;
-  const int64_t slot0 = dense_slot(cut, first, a) * p.piece_floats;
-  auto piece = [&](int i) { return pieces + i * stride + (i == 0 ? slot0 : 0); };
+  const int nth = seq * unit_groups + group, groups_all = p.seqs * unit_groups;
+  auto piece = [&](int i) {
+    return p.pieces + (int64_t(dense_slot(cut, all.run(i), nth, groups_all)) * p.side + member) * p.piece_floats;
+  };
   const int64_t offset = (row0 + row) * D + dim;
   float m = -INFINITY, l = 0.f;  // of row `warp`
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -599,7 +601,7 @@ __global__ void __launch_bounds__(kJoinThreads, 4) dense_join_kernel(const Dense
   if (with_lse && tid < rows) p.lse[out_row + tid] = dense_lse(totals[tid][0], totals[tid][1], Dense16<T>::kLift);
   if (!real || mine > 0) return;
   for (int i = 1; i < groups; ++i) add(1.f, sums[i * columns + column]);
-  const float all = totals[row][1], f = all == 0.f ? 0.f : 1.f / all;
+  const float sum = totals[row][1], f = sum == 0.f ? 0.f : 1.f / sum;
   write(make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
 }
 
@@ -645,15 +647,18 @@ static int dense_sms(int& sms) {
   return rc;
 }
 
-// As many heads to a CTA of the join as leave it with less than four CTAs on an SM, all resident at once; where there are
-// few heads, their dimensions are split.  (32 sequences, 32 heads: a CTA per head and 32 dimensions 17 us, ...)
+// As many heads to a CTA of the join as leave it with eight CTAs on an SM, all resident at once; where there are few
+// heads, their dimensions are split.
 template <typename T, int D>
 static int launch_join(DenseArgs p, cudaStream_t stream) {
-  const int64_t units = int64_t(p.seqs) * p.hkv * p.chunks;
+  const int64_t units = int64_t(p.seqs) * p.hkv * p.chunks, most = 8 * kDenseMaxCtas;
   p.join_rows = 1;
-  p.join_wide = units * p.rows * (D / 32) <= 4 * kDenseMaxCtas ? 32 : D;
+  p.join_wide = D;
+  if (units * p.rows * (D / 32) <= most) p.join_wide = 32;
+  else if (D % 64 == 0 && units * p.rows * (D / 64) <= most) p.join_wide = 64;
+  const auto ctas = [&] { return units * ((p.rows + p.join_rows - 1) / p.join_rows) * (D / p.join_wide); };
   while (p.join_rows < p.rows && 2 * p.join_rows <= kJoinRows && 2 * p.join_rows * p.join_wide / 4 <= kJoinThreads &&
-         units * ((p.rows + p.join_rows - 1) / p.join_rows) * (D / p.join_wide) > 4 * kDenseMaxCtas)
+         ctas() > most)
     p.join_rows *= 2;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(unsigned(units), (p.rows + p.join_rows - 1) / p.join_rows * (D / p.join_wide));
@@ -716,8 +721,8 @@ extern "C" size_t fq_dense_paged_decode_workspace_bytes(int num_seqs, int num_q_
                                                         int head_dim) {
   if (!dense_shape_ok(num_seqs, num_q_heads, num_kv_heads, head_dim)) return 0;
   const DenseGeometry x = dense_geometry(num_q_heads, num_kv_heads, head_dim);
-  const size_t warps = dense_warps(head_dim);
-  return kDensePieces + kDenseMaxCtas * warps * (1 + kDenseTaken) * 2 * size_t(x.piece_floats) * sizeof(float);
+  const int teams = dense_warps(head_dim) / x.side, groups = num_kv_heads * x.chunks / x.side;
+  return kDensePieces + dense_slots(kDenseMaxCtas * teams, num_seqs * groups) * x.side * size_t(x.piece_floats) * sizeof(float);
 }
 
 extern "C" int fq_dense_paged_decode(

@@ -5,11 +5,12 @@
 // of a sequence stand side by side (they are given to warps that run at the same time, so that the heads of a
 // token, which are adjacent in a page, are read together).  The tiles of 16 tokens of all unit groups of all
 // sequences form one list of `total` entries, cut into runs whatever the bounds between sequences are: a ragged
-// batch is balanced.  Where a warp's share is long enough, thirteen sixteenths of the list
-// are dealt out beforehand and the rest in runs of a sixteenth, then a thirty-second, of a share that warps take
-// when they are free: SMs do not get
-// the same share of the memory's bandwidth (8 sequences of 32k - 131k tokens, equal runs: the first SM was
-// through after 345 us, the last after 483).  Where the cuts are never depends on who takes a run.
+// batch is balanced.  Where a warp's share is long enough, thirteen of every sixteen entries are dealt out beforehand
+// and the other three ("tail") in runs of a sixteenth, then a forty-eighth, of a share that warps take when they are
+// free: SMs do not get the same share of the memory's bandwidth (8 sequences of 32k - 131k tokens, equal runs: the
+// first SM was through after 345 us, the last after 483).  Every sequence has its part of the tail, since many short
+// runs are many pieces to join (with the tail at the list's end its last two sequences had 800 each, which took 14 us
+// where the others took 3).  Where the cuts are never depends on who takes a run.
 #pragma once
 
 #include <stdint.h>
@@ -41,53 +42,98 @@ FQ_HD DenseSpan dense_span(int len, int64_t room, int window) {
   return s;
 }
 
+constexpr int kDenseShare = 32;   // tiles of a share from which on there is a tail
+constexpr int kDenseMain = 13;    // entries of sixteen that are not in it
+constexpr int kDenseTaken = 8;    // runs taken per share, at most
+constexpr int kDenseShortest = 2; // tiles of a run at least, where there are enough
+
 struct DenseCut {
-  int total;             // entries of the list
-  int fixed;             // runs that are dealt out beforehand
-  int length, bound;     // of such a run; fixed * length, or total if that is all
-  int medium, length2;   // runs behind `bound`, then
-  int bound2, length3;   // runs behind bound2 to the end
-  FQ_HD int run_of(int at) const {
-    return at < bound ? at / length
-                      : (at < bound2 ? fixed + (at - bound) / length2 : fixed + medium + (at - bound2) / length3);
+  int total;                  // entries of the list (below 2^30)
+  bool split;                 // there is a tail
+  int fixed;                  // runs that are dealt out beforehand, of the others
+  int mains, length;          // entries of these, of one of them
+  int tails;                  // entries of the tail
+  int medium, length2, bound; // runs of the tail's first `bound` entries, their length
+  int length3;                // of a run behind
+
+  // entries of the main kind before entry x of the list, and back from either kind
+  FQ_HD int main_of(int x) const {
+    return split ? x / 16 * kDenseMain + (x % 16 < kDenseMain ? x % 16 : kDenseMain) : x;
+  }
+  FQ_HD int kind_of(bool tail, int x) const { return tail ? x - main_of(x) : main_of(x); }
+  FQ_HD int entry(bool tail, int i) const {
+    return tail ? i / (16 - kDenseMain) * 16 + kDenseMain + i % (16 - kDenseMain)
+                : (split ? i / kDenseMain * 16 + i % kDenseMain : i);
+  }
+  // runs count through; the entries of a run are of its own kind
+  FQ_HD bool is_tail(int run) const { return run >= fixed; }
+  FQ_HD int run_of(bool tail, int i) const {
+    return !tail ? i / length : (i < bound ? fixed + i / length2 : fixed + medium + (i - bound) / length3);
   }
   FQ_HD int begin(int run) const {
-    const int64_t x = run < fixed ? int64_t(run) * length
-                                  : (run < fixed + medium ? bound + int64_t(run - fixed) * length2
-                                                          : bound2 + int64_t(run - fixed - medium) * length3);
-    return x < total ? int(x) : total;
+    if (run < fixed) {
+      const int64_t x = int64_t(run) * length;
+      return x < mains ? int(x) : mains;
+    }
+    const int64_t x = run < fixed + medium ? int64_t(run - fixed) * length2 : bound + int64_t(run - fixed - medium) * length3;
+    return x < tails ? int(x) : tails;
   }
-  FQ_HD int end(int run) const { return begin(run + 1); }
-  FQ_HD int taken() const { return medium + (total - bound2 + length3 - 1) / length3; }
+  FQ_HD int end(int run) const {
+    const int64_t x = int64_t(begin(run)) + (run < fixed ? length : (run < fixed + medium ? length2 : length3));
+    const int most = run < fixed ? mains : tails;
+    return x < most ? int(x) : most;
+  }
+  FQ_HD int taken() const { return split ? medium + (tails - bound + length3 - 1) / length3 : 0; }
 };
-constexpr int kDenseShare = 32;   // tiles of a share from which on a part of the list is taken
-constexpr int kDenseTaken = 6;    // runs taken per share, at most
-constexpr int kDenseShortest = 2; // tiles of a run at least, where there are enough
 FQ_HD DenseCut dense_cut(int total, int fixed) {
   DenseCut c;
-  const int share = (total + fixed - 1) / fixed;  // (total below 2^30)
+  const int share = (total + fixed - 1) / fixed;
   c.total = total;
   c.fixed = fixed;
-  c.length = share < kDenseShortest ? kDenseShortest : share;
-  c.bound = c.bound2 = total;
-  c.medium = 0;
-  c.length2 = c.length3 = 1;
-  if (share < kDenseShare) return c;
+  c.split = share >= kDenseShare;
+  c.mains = c.main_of(total);
+  c.tails = total - c.mains;
+  c.length = c.split ? (c.mains + fixed - 1) / fixed : share;
+  if (c.length < kDenseShortest) c.length = kDenseShortest;
   c.length2 = (share + 15) / 16;
-  c.length3 = (share + 31) / 32;
-  c.length = share - 3 * c.length2;
-  const int64_t bound = int64_t(c.length) * fixed;
-  if (bound >= total) return c;
-  c.bound = int(bound);
-  const int fits = (total - c.bound) / c.length2;
-  c.medium = fits < 2 * fixed ? fits : 2 * fixed;
-  c.bound2 = c.bound + c.medium * c.length2;
+  c.length3 = share < 96 ? 2 : (share + 47) / 48;
+  c.medium = c.tails < fixed * c.length2 ? c.tails / c.length2 : fixed;
+  c.bound = c.medium * c.length2;
   return c;
 }
 
-// A unit group takes the entries [a, b) of the list.  A run that holds all of them writes its result; the
-// others leave a piece.  A run has at most two pieces: of the group that was begun before it (slot 0) and of the
-// one that goes on behind it (slot 1).  The pieces of a group are those of its runs, run_of(a) to run_of(b - 1).
-FQ_HD int dense_slot(const DenseCut& c, int run, int a) { return a < c.begin(run) ? 0 : 1; }
+// A unit group takes the entries [a, b) of the list.  A run that holds all of them writes its result; the others
+// leave a piece.  The pieces of a group are those of its runs, the tail's behind the others.
+struct DensePieces {
+  int main0, mains, tail0, tails;  // first run and number of either kind
+  FQ_HD int count() const { return mains + tails; }
+  FQ_HD int run(int i) const { return i < mains ? main0 + i : tail0 + i - mains; }
+};
+FQ_HD DensePieces dense_pieces(const DenseCut& c, int a, int b) {
+  DensePieces p{0, 0, 0, 0};
+  const int m0 = c.main_of(a), m1 = c.main_of(b), t0 = a - m0, t1 = b - m1;
+  if (m1 > m0) {
+    p.main0 = c.run_of(false, m0);
+    p.mains = c.run_of(false, m1 - 1) - p.main0 + 1;
+  }
+  if (t1 > t0) {
+    p.tail0 = c.run_of(true, t0);
+    p.tails = c.run_of(true, t1 - 1) - p.tail0 + 1;
+  }
+  return p;
+}
+// whether `run`, which holds some of them, holds all
+FQ_HD bool dense_whole(const DenseCut& c, int run, int a, int b) {
+  const bool tail = c.is_tail(run);
+  return c.kind_of(!tail, a) == c.kind_of(!tail, b) && c.kind_of(tail, a) >= c.begin(run) &&
+         c.kind_of(tail, b) <= c.end(run);
+}
+// Where the piece of the `nth` of all `groups` is that a run leaves: along the list of either kind each next piece is
+// of a later run or of a later group, so that the sum of the two counts them.
+FQ_HD int dense_slot(const DenseCut& c, int run, int nth, int groups) {
+  return run + nth + (c.is_tail(run) ? groups : 0);
+}
+// Slots in all, whatever the lengths are: one behind the largest.
+FQ_HD int64_t dense_slots(int fixed, int groups) { return int64_t(fixed) * (1 + kDenseTaken) + 2 * int64_t(groups); }
 
 }  // namespace fq
