@@ -5,9 +5,15 @@
 // Angles are taken in 64 bits: at position 10^6 an angle of 32 bits is off by 0.03.  In turns (position * frequency
 // / 2 pi) the whole ones are dropped there, what is left goes through sincospif in 32 bits.
 //
-// Bound: HBM, every row is read and written once.  A CTA takes a few tokens: their angles go to shared memory
-// once (the heads of a token share them), then every thread turns vectors of 16 bytes, all loads of a thread before
-// its first store.
+// Bound: HBM, every row is read and written once.  As many CTAs as there is room for go through the tokens, a few at a
+// time.  Each time they find what the heads of those tokens share, the angles and where their rows in the pages are,
+// in shared memory.  Every warp has a job, some heads of q, k or v: which tensor it works on is the same for all its
+// lanes, a lane keeps its place (16 bytes, or two times 16 that make pairs) in the same rows of each token, goes on by a
+// stride, and has the next token's on the way before it stores this one's, the next angles being found meanwhile.
+// (With rows of all three tensors dealt to the threads of a CTA the same work took 240 instructions to a place and
+// three times as long.)
+#include <algorithm>
+
 #include "fq_common.cuh"
 
 namespace fq {
@@ -30,7 +36,8 @@ struct RotaryArgs {
   float scale, sign;
 };
 
-constexpr int kRotThreads = 256;
+constexpr int kRotWarps = 8;   // of a CTA at most
+constexpr int kRotTokens = 4;  // at a time, at most
 
 // (a cos - b sin, b cos + a sin), rounded the same way in every variant
 __device__ __forceinline__ float2 turn(float a, float b, float2 cs) {
@@ -42,92 +49,187 @@ struct alignas(sizeof(T) * N) Vec {
   T v[N];
 };
 
-// N values to a vector; pairs of a work item: N in the half layout (two vectors), N / 2 or one in the other
+struct RotaryPlace {
+  int64_t k, v;         // append: offsets of the token's rows
+  bool placed, stored;  // its position is not negative; it has a slot
+};
+
+// The jobs of a tensor: `rows` rows to a lane, 32 / places side by side, further jobs for places beyond 32.
+struct RotaryJobs {
+  int places, side, parts, count;
+  __host__ __device__ RotaryJobs(int all, int heads, int rows)
+      : places(all < 32 ? all : 32), side(32 / places), parts((all + 31) / 32),
+        count((heads + rows * side - 1) / (rows * side) * parts) {}
+};
+// Places of a row of q or k (v: without a part that is turned), the values of a place in one vector or in two.
+__host__ __device__ inline bool rotary_two(int n, bool half_layout) { return half_layout || n == 1; }
+__host__ __device__ inline int rotary_places(int n, bool half_layout, int head_dim, int rotary_dim) {
+  return rotary_dim / (rotary_two(n, half_layout) ? 2 * n : n) + (head_dim - rotary_dim) / n;
+}
+__host__ __device__ inline int rotary_rows(int n, bool half_layout) { return rotary_two(n, half_layout) ? 2 : 4; }
+
+// values 2 k and 2 k + 1 of a vector
+template <typename T, int N>
+__device__ __forceinline__ float2 get2(const Vec<T, N>& x, int k) {
+  if constexpr (sizeof(T) == 4) {
+    return make_float2(x.v[2 * k], x.v[2 * k + 1]);
+  } else {
+    float y[2];
+    load2(x.v + 2 * k, y);
+    return make_float2(y[0], y[1]);
+  }
+}
+__device__ __forceinline__ void put2(float* at, float x, float y) { at[0] = x; at[1] = y; }
+__device__ __forceinline__ void put2(__half* at, float x, float y) {
+  *reinterpret_cast<__half2*>(at) = __floats2half2_rn(x, y);
+}
+__device__ __forceinline__ void put2(__nv_bfloat16* at, float x, float y) {
+  *reinterpret_cast<__nv_bfloat162*>(at) = __floats2bfloat162_rn(x, y);
+}
+
+// N values to a vector.  HALF: pairs half a rotated part apart, else adjacent.
 template <typename T, int N, bool HALF>
-__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs p, int per_cta) {
-  extern __shared__ float2 angles[];  // [per_cta][rotary_dim / 2]
-  __shared__ int64_t place[64];       // where a token's row goes; -1: nowhere
-  const int tid = threadIdx.x;
-  const int64_t token0 = int64_t(blockIdx.x) * per_cta;
-  const int count = int(p.tokens - token0 < per_cta ? p.tokens - token0 : per_cta);
-  const int half = p.rotary_dim / 2;
-
-  auto position = [&](int64_t i) -> int64_t {
-    return p.positions64 ? static_cast<const int64_t*>(p.positions)[i] : static_cast<const int32_t*>(p.positions)[i];
+__global__ void __launch_bounds__(kRotWarps * 32, 3) rotary_kernel(const RotaryArgs p, int batch) {
+  using V = Vec<T, N>;
+  constexpr int kPairs = HALF ? N : (N > 1 ? N / 2 : 1), kRows = HALF || N == 1 ? 2 : 4;
+  constexpr bool kTwo = HALF || N == 1;  // the values of a place stand in two vectors
+  // [2][batch][chunk][place][2]: the cosines and sines of a place are read two at a time, adjacent places together
+  extern __shared__ __align__(16) float2 angles[];
+  constexpr int kChunk = kPairs > 1 ? 2 : 1;
+  __shared__ RotaryPlace where[2][kRotTokens];
+  const int half = p.rotary_dim / 2, turns_of = half / kPairs;
+  const int tid = threadIdx.x, lane = tid & 31;
+  auto integer = [](const void* x, int wide, int64_t i) -> int64_t {
+    return wide ? static_cast<const int64_t*>(x)[i] : static_cast<const int32_t*>(x)[i];
   };
-  for (int i = tid; i < count * half; i += kRotThreads) {
-    const int token = i / half, j = i - token * half;
-    const double turns = double(position(token0 + token)) * (p.freq[j] * 0.15915494309189535);
-    float s, c;
-    sincospif(float(2.0 * (turns - rint(turns))), &s, &c);
-    angles[i] = make_float2(c * p.scale, s * p.scale * p.sign);
-  }
-  for (int i = tid; i < count; i += kRotThreads) {
-    int64_t to = token0 + i;
-    if (p.positions && position(to) < 0) to = -1;  // (q and k of such a row are not touched)
-    place[i] = to;
-  }
-  __syncthreads();
-
-  const int pairs = HALF ? N : (N > 1 ? N / 2 : 1);
-  const int turn_items = half / pairs;
-  const int keep_items = (p.head_dim - p.rotary_dim) / N;
-  const int items = turn_items + keep_items, all_items = p.head_dim / N;
-  const int turned = (p.q.heads + p.k.heads) * items;
-  const int total = turned + p.v.heads * all_items;
-  for (int token = 0; token < count; ++token) {
-    const int64_t from = token0 + token;
-    int64_t slot = from;
-    if (p.slots)
-      slot = p.slots64 ? static_cast<const int64_t*>(p.slots)[from] : static_cast<const int32_t*>(p.slots)[from];
-    const bool stored = !p.slots || (slot >= 0 && slot < p.num_slots);
-    for (int i = tid; i < total; i += kRotThreads) {
-      const bool is_v = i >= turned;
-      const int per_head = is_v ? all_items : items;
-      const int x = is_v ? i - turned : i;
-      int head = x / per_head;
-      const int item = x - head * per_head;
-      const bool is_k = !is_v && head >= p.q.heads;
-      if (is_k) head -= p.q.heads;
-      const RotaryTensor& t = is_v ? p.v : (is_k ? p.k : p.q);
-      if (!is_v && place[token] < 0) continue;
-      if ((is_k || is_v) && !stored) continue;
-      const T* src = static_cast<const T*>(t.src) + from * t.src_token + head * t.src_head;
-      T* dst = static_cast<T*>(t.dst) + head * t.dst_head;
-      if ((is_k || is_v) && p.slots)
-        dst += slot / p.block_size * (is_v ? p.v_block : p.k_block) + slot % p.block_size * t.dst_token;
-      else
-        dst += from * t.dst_token;
-      using V = Vec<T, N>;
-      if (is_v || item >= turn_items) {
-        const int at = is_v ? item * N : p.rotary_dim + (item - turn_items) * N;
-        if (dst != src) *reinterpret_cast<V*>(dst + at) = *reinterpret_cast<const V*>(src + at);
-        continue;
+  auto prepare = [&](int64_t token0, int count, int buffer) {
+    for (int i = tid; i < half * count; i += blockDim.x) {
+      const int of = i / half, j = i - of * half;
+      const double turns = double(integer(p.positions, p.positions64, token0 + of)) * (p.freq[j] * 0.15915494309189535);
+      float s, c;
+      sincospif(float(2.0 * (turns - rint(turns))), &s, &c);
+      const int place = j / kPairs, e = j % kPairs;
+      angles[(buffer * batch + of) * half + (e / kChunk * turns_of + place) * kChunk + e % kChunk] =
+          make_float2(c * p.scale, s * p.scale * p.sign);
+    }
+    if (tid < count) {
+      RotaryPlace w{0, 0, true, true};
+      if (p.positions) w.placed = integer(p.positions, p.positions64, token0 + tid) >= 0;
+      if (p.slots) {
+        const int64_t slot = integer(p.slots, p.slots64, token0 + tid);
+        w.stored = slot >= 0 && slot < p.num_slots;
+        const int64_t block = w.stored ? slot / p.block_size : 0, row = w.stored ? slot - block * p.block_size : 0;
+        w.k = block * p.k_block + row * p.k.dst_token;
+        w.v = block * p.v_block + row * p.v.dst_token;
       }
-      const float2* cs = angles + token * half + item * pairs;
-      if constexpr (HALF) {
-        V a = *reinterpret_cast<const V*>(src + item * N), b = *reinterpret_cast<const V*>(src + half + item * N);
+      where[buffer][tid] = w;
+    }
+  };
+
+  // ---- this warp's job ---------------------------------------------------------------------------------
+  const int all = rotary_places(N, HALF, p.head_dim, p.rotary_dim);
+  const bool halves = kTwo && p.head_dim % (2 * N) == 0;  // of a row of v, copied by places like those that are turned
+  const int all_v = p.head_dim / (halves ? 2 * N : N);
+  const RotaryJobs jq(all, p.q.heads, kRows), jk(all, p.k.heads, kRows), jv(all_v, p.v.heads, kRows);
+  int job = blockIdx.y * (blockDim.x / 32) + __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const int kind = job < jq.count ? 0 : (job < jq.count + jk.count ? 1 : 2);
+  if (kind > 0) job -= jq.count;
+  if (kind > 1) job -= jk.count;
+  const RotaryTensor& t = kind == 2 ? p.v : (kind == 1 ? p.k : p.q);
+  const RotaryJobs& j = kind == 2 ? jv : (kind == 1 ? jk : jq);
+  const bool working = job < j.count;
+  const int row = lane / j.places, place = job % j.parts * 32 + lane - row * j.places;
+  const int head = job / j.parts * kRows * j.side + row;
+  const bool turned = kind < 2 && place < turns_of;
+  const bool two = kind == 2 ? halves : kTwo && turned;
+  const int rows = !working || row >= j.side || place >= (kind == 2 ? all_v : all) || head >= t.heads
+                       ? 0
+                       : min(kRows, (t.heads - head + j.side - 1) / j.side);
+  int at = place * N, too = 0;  // the values of a place; how far its second vector is behind the first
+  if (kind == 2) {
+    too = p.head_dim / 2;
+  } else if (!turned) {
+    at = p.rotary_dim + (place - turns_of) * N;
+  } else if (kTwo) {
+    if (!HALF) at = 2 * place;
+    too = HALF ? half : 1;
+  }
+  const bool paged = p.slots && kind > 0;
+  const T* const src = static_cast<const T*>(t.src) + head * t.src_head + at;
+  T* const dst = static_cast<T*>(t.dst) + head * t.dst_head + at;
+  const int64_t src_row = j.side * t.src_head, dst_row = j.side * t.dst_head;
+
+  V a[kRows], b[kTwo ? kRows : 1];
+  auto load = [&](int64_t token, V (&u)[kRows], V (&w)[kTwo ? kRows : 1]) {
+    const T* x = src + token * t.src_token;
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float2 y = turn(to_f32(a.v[e]), to_f32(b.v[e]), cs[e]);
-          a.v[e] = from_f32<T>(y.x);
-          b.v[e] = from_f32<T>(y.y);
-        }
-        *reinterpret_cast<V*>(dst + item * N) = a;
-        *reinterpret_cast<V*>(dst + half + item * N) = b;
-      } else if constexpr (N > 1) {
-        V a = *reinterpret_cast<const V*>(src + item * N);
+    for (int r = 0; r < kRows; ++r) {
+      if (r >= rows) break;
+      u[r] = *reinterpret_cast<const V*>(x + r * src_row);
+      if (kTwo && two) w[r] = *reinterpret_cast<const V*>(x + r * src_row + too);
+    }
+  };
+  const int64_t step = int64_t(gridDim.x) * batch;
+  int64_t token0 = int64_t(blockIdx.x) * batch;
+  if (token0 < p.tokens) load(token0, a, b);
+  for (int buffer = 0; token0 < p.tokens; token0 += step, buffer ^= 1) {
+    const int count = int(p.tokens - token0 < batch ? p.tokens - token0 : batch);
+    prepare(token0, count, buffer);
+    __syncthreads();
+    for (int i = 0; i < count; ++i) {
+      V next_a[kRows], next_b[kTwo ? kRows : 1];
+      const int64_t next = i + 1 < count ? token0 + i + 1 : token0 + step;
+      if (next < p.tokens) load(next, next_a, next_b);
+      const RotaryPlace& w = where[buffer][i];
+      if ((kind == 2 || w.placed) && (kind == 0 || w.stored)) {
+        if (turned) {
+          float2 cs[kPairs];
+          const float2* c = angles + (buffer * batch + i) * half + place * kChunk;
 #pragma unroll
-        for (int e = 0; e < N; e += 2) {
-          const float2 y = turn(to_f32(a.v[e]), to_f32(a.v[e + 1]), cs[e / 2]);
-          a.v[e] = from_f32<T>(y.x);
-          a.v[e + 1] = from_f32<T>(y.y);
+          for (int e = 0; e < kPairs; e += kChunk) {
+            if constexpr (kChunk == 2) {
+              const float4 x = *reinterpret_cast<const float4*>(c + e * turns_of);
+              cs[e] = make_float2(x.x, x.y);
+              cs[e + 1] = make_float2(x.z, x.w);
+            } else {
+              cs[e] = c[e * turns_of];
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < kRows; ++r) {
+            if constexpr (N == 1) {
+              const float2 y = turn(to_f32(a[r].v[0]), to_f32(b[r].v[0]), cs[0]);
+              a[r].v[0] = from_f32<T>(y.x);
+              b[r].v[0] = from_f32<T>(y.y);
+            } else if constexpr (HALF) {
+#pragma unroll
+              for (int k = 0; k < N / 2; ++k) {
+                const float2 u = get2(a[r], k), v = get2(b[r], k);
+                const float2 y = turn(u.x, v.x, cs[2 * k]), z = turn(u.y, v.y, cs[2 * k + 1]);
+                put2(a[r].v + 2 * k, y.x, z.x);
+                put2(b[r].v + 2 * k, y.y, z.y);
+              }
+            } else {
+#pragma unroll
+              for (int k = 0; k < N / 2; ++k) {
+                const float2 u = get2(a[r], k), y = turn(u.x, u.y, cs[k]);
+                put2(a[r].v + 2 * k, y.x, y.y);
+              }
+            }
+          }
         }
-        *reinterpret_cast<V*>(dst + item * N) = a;
-      } else {
-        const float2 y = turn(to_f32(src[2 * item]), to_f32(src[2 * item + 1]), *cs);
-        dst[2 * item] = from_f32<T>(y.x);
-        dst[2 * item + 1] = from_f32<T>(y.y);
+        T* y = dst + (paged ? (kind == 2 ? w.v : w.k) : (token0 + i) * t.dst_token);
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          if (r >= rows) break;
+          *reinterpret_cast<V*>(y + r * dst_row) = a[r];
+          if (kTwo && two) *reinterpret_cast<V*>(y + r * dst_row + too) = b[r];
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        a[r] = next_a[r];
+        if (kTwo) b[r] = next_b[r];
       }
     }
   }
@@ -141,18 +243,27 @@ static bool rows_aligned(const RotaryTensor& t, size_t size, bool src, bool dst)
 template <typename T>
 static int launch_rotary(const RotaryArgs& p, bool half_layout, cudaStream_t stream) {
   constexpr int N = 16 / sizeof(T);
-  const int per_cta = p.tokens <= 592 ? 1 : 4;
-  const int64_t ctas = (p.tokens + per_cta - 1) / per_cta;
-  FQ_REQUIRE(ctas <= 0x7fffffff, FQ_ERR_UNSUPPORTED, "rotary: too many tokens");
-  const size_t smem = size_t(per_cta) * (p.rotary_dim / 2) * sizeof(float2);
   const bool wide = rows_aligned(p.q, sizeof(T), true, true) && rows_aligned(p.k, sizeof(T), true, true) &&
                     rows_aligned(p.v, sizeof(T), true, true) && (p.k_block | p.v_block) * int64_t(sizeof(T)) % 16 == 0 &&
                     p.head_dim % N == 0 && p.rotary_dim % (half_layout ? 2 * N : N) == 0;
-  const dim3 grid = dim3(unsigned(ctas));
-  if (wide && half_layout) rotary_kernel<T, N, true><<<grid, kRotThreads, smem, stream>>>(p, per_cta);
-  else if (wide) rotary_kernel<T, N, false><<<grid, kRotThreads, smem, stream>>>(p, per_cta);
-  else if (half_layout) rotary_kernel<T, 1, true><<<grid, kRotThreads, smem, stream>>>(p, per_cta);
-  else rotary_kernel<T, 1, false><<<grid, kRotThreads, smem, stream>>>(p, per_cta);
+  const int n = wide ? N : 1, rows = rotary_rows(n, half_layout);
+  const int all = rotary_places(n, half_layout, p.head_dim, p.rotary_dim);
+  const int all_v = p.head_dim / (rotary_two(n, half_layout) && p.head_dim % (2 * n) == 0 ? 2 * n : n);
+  const int jobs = RotaryJobs(all, p.q.heads, rows).count + RotaryJobs(all, p.k.heads, rows).count +
+                   RotaryJobs(all_v, p.v.heads, rows).count;
+  const int groups = (jobs + kRotWarps - 1) / kRotWarps, warps = (jobs + groups - 1) / groups;
+  // A few tokens are spread over more CTAs, one at a time.
+  const int batch = p.tokens <= 592 ? 1 : kRotTokens;
+  const size_t smem = 2 * size_t(batch) * (p.rotary_dim / 2) * sizeof(float2);
+  const auto kernel = wide ? (half_layout ? rotary_kernel<T, N, true> : rotary_kernel<T, N, false>)
+                           : (half_layout ? rotary_kernel<T, 1, true> : rotary_kernel<T, 1, false>);
+  int device = 0, sms = 0, fit = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+  if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, warps * 32, smem);
+  if (e != cudaSuccess) return fail(FQ_ERR_CUDA, "rotary: %s", cudaGetErrorString(e));
+  const int64_t ctas = std::min<int64_t>((p.tokens + batch - 1) / batch, std::max(1, sms * fit / groups));
+  kernel<<<dim3(unsigned(ctas), groups), warps * 32, smem, stream>>>(p, batch);
   return check_launch("rotary");
 }
 

@@ -13,7 +13,8 @@ namespace fq {
 
 namespace cg = cooperative_groups;
 
-constexpr int kPlanThreads = 512;
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanBatch = 4;  // pages or tokens of a thread whose loads are in flight together
 constexpr int kPlanMaxRequests = 4096;
 
 struct PlanArgs {
@@ -161,26 +162,49 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanArgs 
 
   // ---- pages off the stack ------------------------------------------------------------------------------
   const int64_t first = int64_t(cta) * kPlanThreads + tid, step = int64_t(ctas) * kPlanThreads;
-  for (int64_t x = first; x < all_pages; x += step) {
-    const int i = plan_owner(taken, some, int32_t(x));
-    const PlanRequest r = plan_request(p, i);
-    p.table[i * p.table_stride + r.have + (x - taken[i])] = p.free_pages[height - 1 - x];
+  for (int64_t x0 = first; x0 < all_pages; x0 += kPlanBatch * step) {
+    int32_t id[kPlanBatch], context[kPlanBatch];
+    int owner[kPlanBatch];
+#pragma unroll
+    for (int k = 0; k < kPlanBatch; ++k) {
+      const int64_t x = x0 + k * step;
+      if (x >= all_pages) continue;
+      owner[k] = plan_owner(taken, some, int32_t(x));
+      context[k] = p.context[owner[k]];
+      id[k] = p.free_pages[height - 1 - x];
+    }
+#pragma unroll
+    for (int k = 0; k < kPlanBatch; ++k) {
+      const int64_t x = x0 + k * step;
+      if (x >= all_pages) continue;
+      const uint32_t have = (uint32_t(context[k]) + p.block_size - 1) / p.block_size;
+      p.table[owner[k] * p.table_stride + have + (x - taken[owner[k]])] = id[k];
+    }
   }
   // ---- slots and positions: a page that was taken just now is read off the stack, not from the table -------
-  for (int64_t x = first; x < p.room; x += step) {
-    int64_t slot = -1, at = -1;
-    if (x < all_tokens) {
+  for (int64_t x0 = first; x0 < p.room; x0 += kPlanBatch * step) {
+    int64_t slot[kPlanBatch], at[kPlanBatch];
+    const uint32_t bs = p.block_size;
+#pragma unroll
+    for (int k = 0; k < kPlanBatch; ++k) {
+      const int64_t x = x0 + k * step;
+      slot[k] = at[k] = -1;
+      if (x >= all_tokens) continue;
       const int i = plan_owner(starts, some, int32_t(x));
-      const uint32_t bs = p.block_size, context = p.context[i];
-      const uint32_t position = context + uint32_t(x - starts[i]);
+      const uint32_t context = p.context[i], position = context + uint32_t(x - starts[i]);
       const uint32_t page = position / bs, have = (context + bs - 1) / bs;
       const int32_t id = page < have ? p.table[i * p.table_stride + page]
                                      : p.free_pages[height - 1 - (taken[i] + int64_t(page - have))];
-      slot = int64_t(id) * bs + (position - page * bs);
-      at = position;
+      slot[k] = int64_t(id) * bs + (position - page * bs);
+      at[k] = position;
     }
-    p.slots[x] = slot;
-    p.positions[x] = at;
+#pragma unroll
+    for (int k = 0; k < kPlanBatch; ++k) {
+      const int64_t x = x0 + k * step;
+      if (x >= p.room) break;
+      p.slots[x] = slot[k];
+      p.positions[x] = at[k];
+    }
   }
   cg::this_cluster().sync();  // free_count may be count_out
   if (cta == 0 && tid == 0) *p.count_out = int32_t(height - all_pages);
@@ -227,9 +251,21 @@ __global__ void __launch_bounds__(kPlanThreads) release_pages_kernel(const Relea
   }
   __syncthreads();
   const int64_t total = all_pages < space ? all_pages : space;
-  for (int64_t x = int64_t(cta) * kPlanThreads + tid; x < total; x += int64_t(ctas) * kPlanThreads) {
-    const int i = plan_owner(starts, p.requests, int32_t(x));
-    p.free_pages[height + x] = p.table[i * p.table_stride + (x - starts[i])];
+  const int64_t step = int64_t(ctas) * kPlanThreads;
+  for (int64_t x0 = int64_t(cta) * kPlanThreads + tid; x0 < total; x0 += kPlanBatch * step) {
+    int32_t id[kPlanBatch];
+#pragma unroll
+    for (int k = 0; k < kPlanBatch; ++k) {
+      const int64_t x = x0 + k * step;
+      if (x >= total) continue;
+      const int i = plan_owner(starts, p.requests, int32_t(x));
+      id[k] = p.table[i * p.table_stride + (x - starts[i])];
+    }
+#pragma unroll
+    for (int k = 0; k < kPlanBatch; ++k) {
+      const int64_t x = x0 + k * step;
+      if (x < total) p.free_pages[height + x] = id[k];
+    }
   }
   cg::this_cluster().sync();
   if (cta == 0 && tid == 0) *p.count_out = int32_t(height + total);
