@@ -252,17 +252,22 @@ static int launch_rotary(const RotaryArgs& p, bool half_layout, cudaStream_t str
   const int jobs = RotaryJobs(all, p.q.heads, rows).count + RotaryJobs(all, p.k.heads, rows).count +
                    RotaryJobs(all_v, p.v.heads, rows).count;
   const int groups = (jobs + kRotWarps - 1) / kRotWarps, warps = (jobs + groups - 1) / groups;
-  // A few tokens are spread over more CTAs, one at a time.
-  const int batch = p.tokens <= 592 ? 1 : kRotTokens;
+  // A few tokens are spread over more CTAs.  (590 tokens of 40 heads: 4.3, 4.1, 5.3 us with 1, 2, 4 at a time, 148: 3.1,
+  // 3.8, 5.2, 8192: 35.1, 32.2, 32.7, 16384: 66.2, 60.6, 58.4.)
+  const int batch = p.tokens <= 592 ? 1 : (p.tokens <= 1184 ? 2 : kRotTokens);
   const size_t smem = 2 * size_t(batch) * (p.rotary_dim / 2) * sizeof(float2);
   const auto kernel = wide ? (half_layout ? rotary_kernel<T, N, true> : rotary_kernel<T, N, false>)
                            : (half_layout ? rotary_kernel<T, 1, true> : rotary_kernel<T, 1, false>);
-  int device = 0, sms = 0, fit = 0;
-  cudaError_t e = cudaGetDevice(&device);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-  if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, warps * 32, smem);
-  if (e != cudaSuccess) return fail(FQ_ERR_CUDA, "rotary: %s", cudaGetErrorString(e));
-  const int64_t ctas = std::min<int64_t>((p.tokens + batch - 1) / batch, std::max(1, sms * fit / groups));
+  // no more CTAs than are resident together
+  int64_t ctas = (p.tokens + batch - 1) / batch;
+  if (ctas > 64) {
+    int device = 0, sms = 0, fit = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, warps * 32, smem);
+    if (e != cudaSuccess) return fail(FQ_ERR_CUDA, "rotary: %s", cudaGetErrorString(e));
+    ctas = std::min<int64_t>(ctas, std::max(1, sms * fit / groups));
+  }
   kernel<<<dim3(unsigned(ctas), groups), warps * 32, smem, stream>>>(p, batch);
   return check_launch("rotary");
 }

@@ -2,9 +2,12 @@
 // finished requests.  Free pages are a stack in global memory; requests take from its top in their order.
 //
 // Bound: latency for a decode step (a few KB), the slots and positions written (16 bytes a token) for a prefill
-// step.  One launch of one cluster: every CTA of it finds the prefix sums over the requests for itself (8 bytes a
-// request from the L2, no exchange), then takes a share of the pages and tokens.  The stack's height may be updated
-// in place: it is written behind a barrier of the cluster that all have read it before.
+// step.  One launch: every CTA finds the prefix sums over the requests for itself (8 bytes a request from the L2, no
+// exchange), then takes a share of the pages and tokens.  Where the stack's height is updated in place it must not be
+// written before all CTAs have read it: then they are one cluster, which has a barrier; else as many as there is work
+// for.
+#include <algorithm>
+
 #include <cooperative_groups.h>
 
 #include "fq_common.cuh"
@@ -52,29 +55,40 @@ __device__ __forceinline__ void plan_before(int64_t& x, int64_t& y, int64_t (*su
   __syncthreads();
   x = a - x;
   y = b - y;
-  for (int w = 0; w < warp; ++w) {
-    x += sums[w][0];
-    y += sums[w][1];
+  int64_t u = lane < warp ? sums[lane][0] : 0, w = lane < warp ? sums[lane][1] : 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    u += __shfl_xor_sync(0xffffffffu, u, o);
+    w += __shfl_xor_sync(0xffffffffu, w, o);
   }
+  x += u;
+  y += w;
 }
+static_assert(kPlanThreads == 1024, "a lane to a warp's sums");
 
 // A request as it is treated: a negative length or more pages than a row of the block table holds make it
 // invalid, which counts as one without tokens.
 struct PlanRequest {
-  int64_t context, query;  // (query: 0 where invalid)
-  int64_t have, grow;      // pages it holds, pages it takes
+  int32_t context, query;  // (query: 0 where invalid)
+  int32_t grow;            // pages it takes
   bool valid;
 };
+__device__ __forceinline__ uint32_t plan_pages(uint32_t tokens, uint32_t block_size) {
+  const uint32_t n = tokens / block_size;
+  return n + (n * block_size != tokens);
+}
 __device__ __forceinline__ PlanRequest plan_request(const PlanArgs& p, int i) {
   PlanRequest r;
-  const int64_t bs = p.block_size;
   r.context = p.context[i];
   r.query = p.query[i];
-  const int64_t need = (r.context + r.query + bs - 1) / bs;
-  r.valid = r.context >= 0 && r.query >= 0 && need <= p.width;
+  r.valid = r.context >= 0 && r.query >= 0;
+  r.grow = 0;
+  if (r.valid) {  // (the sum of both fits into 32 bits without a sign)
+    const uint32_t need = plan_pages(uint32_t(r.context) + uint32_t(r.query), p.block_size);
+    r.valid = need <= uint32_t(p.width);
+    if (r.valid && r.query > 0) r.grow = need - plan_pages(r.context, p.block_size);
+  }
   if (!r.valid) r.query = 0;
-  r.have = r.valid ? (r.context + bs - 1) / bs : 0;
-  r.grow = r.query > 0 ? need - r.have : 0;
   return r;
 }
 
@@ -105,9 +119,12 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanArgs 
   if (tid == 0) cut = p.requests;
   const int each = (p.requests + kPlanThreads - 1) / kPlanThreads;
   const int i0 = min(tid * each, p.requests), i1 = min(i0 + each, p.requests);
+  PlanRequest mine{};  // (kept: up to 1024 requests each thread has one)
+  if (i0 < i1) mine = plan_request(p, i0);
+  auto request = [&](int i) { return i == i0 ? mine : plan_request(p, i); };
   int64_t tokens = 0, pages = 0;
   for (int i = i0; i < i1; ++i) {
-    const PlanRequest r = plan_request(p, i);
+    const PlanRequest r = request(i);
     tokens += r.query;
     pages += r.grow;
   }
@@ -115,7 +132,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanArgs 
   {
     int64_t t = tokens, g = pages;
     for (int i = i0; i < i1; ++i) {
-      const PlanRequest r = plan_request(p, i);
+      const PlanRequest r = request(i);
       t += r.query;
       g += r.grow;
       if (r.query > 0 && (t > p.room || g > height)) {
@@ -126,7 +143,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanArgs 
   }
   __syncthreads();
   for (int i = i0; i < i1; ++i) {
-    const PlanRequest r = plan_request(p, i);
+    const PlanRequest r = request(i);
     if (i <= cut) {  // (fits into 32 bits: all before `cut` do)
       starts[i] = int32_t(tokens);
       taken[i] = int32_t(pages);
@@ -152,7 +169,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanArgs 
   for (int i = cta * kPlanThreads + tid; i < p.requests; i += ctas * kPlanThreads) {
     const PlanRequest r = plan_request(p, i);
     const bool served = r.valid && (r.query == 0 || i < cut);
-    int64_t len = r.context < 0 ? 0 : (r.context > most ? most : r.context);
+    int64_t len = r.context < 0 ? 0 : (r.context > most ? most : int64_t(r.context));
     if (served) len += r.query;
     p.seq_lens[i] = int32_t(len);
     p.starts[i] = i < some ? starts[i] : all_tokens;
@@ -177,7 +194,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanArgs 
     for (int k = 0; k < kPlanBatch; ++k) {
       const int64_t x = x0 + k * step;
       if (x >= all_pages) continue;
-      const uint32_t have = (uint32_t(context[k]) + p.block_size - 1) / p.block_size;
+      const uint32_t have = plan_pages(context[k], p.block_size);
       p.table[owner[k] * p.table_stride + have + (x - taken[owner[k]])] = id[k];
     }
   }
@@ -192,7 +209,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanArgs 
       if (x >= all_tokens) continue;
       const int i = plan_owner(starts, some, int32_t(x));
       const uint32_t context = p.context[i], position = context + uint32_t(x - starts[i]);
-      const uint32_t page = position / bs, have = (context + bs - 1) / bs;
+      const uint32_t page = position / bs, have = plan_pages(context, bs);
       const int32_t id = page < have ? p.table[i * p.table_stride + page]
                                      : p.free_pages[height - 1 - (taken[i] + int64_t(page - have))];
       slot[k] = int64_t(id) * bs + (position - page * bs);
@@ -206,7 +223,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanArgs 
       p.positions[x] = at[k];
     }
   }
-  cg::this_cluster().sync();  // free_count may be count_out
+  cg::this_cluster().sync();  // (of one CTA, unless free_count is count_out)
   if (cta == 0 && tid == 0) *p.count_out = int32_t(height - all_pages);
 }
 
@@ -232,10 +249,9 @@ __global__ void __launch_bounds__(kPlanThreads) release_pages_kernel(const Relea
   int64_t height = *p.free_count;
   height = height < 0 ? 0 : (height > p.capacity ? p.capacity : height);
   auto pages_of = [&](int i) -> int64_t {
-    const int64_t context = p.context[i];
+    const int32_t context = p.context[i];
     if (!p.finished[i] || context <= 0) return 0;
-    const int64_t n = (context + p.block_size - 1) / p.block_size;
-    return n < p.width ? n : p.width;
+    return min(plan_pages(context, p.block_size), uint32_t(p.width));
   };
   const int each = (p.requests + kPlanThreads - 1) / kPlanThreads;
   const int i0 = min(tid * each, p.requests), i1 = min(i0 + each, p.requests);
@@ -271,9 +287,14 @@ __global__ void __launch_bounds__(kPlanThreads) release_pages_kernel(const Relea
   if (cta == 0 && tid == 0) *p.count_out = int32_t(height + total);
 }
 
+constexpr int kPlanCluster = 8, kPlanMaxCtas = 148;
+// `work`: pages or tokens
 template <typename Args>
-static int launch_plan(void (*kernel)(Args), const Args& p, int ctas, size_t smem, const char* what,
+static int launch_plan(void (*kernel)(Args), const Args& p, int64_t work, size_t smem, const char* what,
                        cudaStream_t stream) {
+  int ctas = int(std::min<int64_t>(std::max<int64_t>(1, (work + kPlanThreads - 1) / kPlanThreads), kPlanMaxCtas));
+  const bool in_place = p.count_out == p.free_count;
+  if (in_place && ctas > 1) ctas = kPlanCluster;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(ctas);
   config.blockDim = dim3(kPlanThreads);
@@ -284,7 +305,7 @@ static int launch_plan(void (*kernel)(Args), const Args& p, int ctas, size_t sme
   cluster.val.clusterDim.x = ctas;
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   config.attrs = &cluster;
-  config.numAttrs = 1;
+  config.numAttrs = in_place && ctas > 1 ? 1 : 0;
   const cudaError_t e = cudaLaunchKernelEx(&config, kernel, p);
   if (e != cudaSuccess) return fail(FQ_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   return check_launch(what);
@@ -327,8 +348,7 @@ extern "C" int fq_plan_paged_step(const int32_t* context_lens, const int32_t* qu
   p.seq_lens = seq_lens; p.starts = cu_seqlens_q;
   p.slots = slot_mapping; p.positions = positions;
   p.served = served; p.count_out = free_count_out;
-  const int ctas = max_tokens <= 4 * kPlanThreads ? 1 : 8;
-  return launch_plan(plan_step_kernel, p, ctas, 2 * size_t(num_requests) * sizeof(int32_t), "step plan", stream);
+  return launch_plan(plan_step_kernel, p, max_tokens, 2 * size_t(num_requests) * sizeof(int32_t), "step plan", stream);
 }
 
 extern "C" int fq_release_pages(const uint8_t* finished, const int32_t* context_lens, int num_requests,
@@ -346,7 +366,6 @@ extern "C" int fq_release_pages(const uint8_t* finished, const int32_t* context_
   p.requests = num_requests; p.block_size = block_size;
   p.free_pages = free_blocks; p.capacity = free_capacity; p.free_count = free_count;
   p.count_out = free_count_out;
-  const int64_t most = int64_t(num_requests) * block_table_width;
-  const int ctas = most <= 4 * kPlanThreads ? 1 : 8;
-  return launch_plan(release_pages_kernel, p, ctas, size_t(num_requests) * sizeof(int32_t), "release", stream);
+  return launch_plan(release_pages_kernel, p, std::min(int64_t(num_requests) * block_table_width, free_capacity),
+                     size_t(num_requests) * sizeof(int32_t), "release", stream);
 }
