@@ -195,18 +195,21 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
   const int here = blockIdx.x * S::kWarps + warp;
   int run = here / p.side, member = here - run * p.side;
   int at = cut.begin(run), end = cut.end(run);
-  uint32_t ticket = 0;  // (lane 0) the next run
-  auto take = [&] {
+  uint32_t ticket = 0;  // (lane 0) the next run, where it has been asked for
+  bool asked = false;
+  auto ask = [&] {
     if (taken && lane == 0) ticket = atomicAdd(p.tickets, 1u);
+    asked = true;
   };
-  take();
   int made = 0, issued = 0, used = 0;  // tiles described, on their way, done
   int waiting = 0;                     // described in `next`, not stored yet
   bool finished = false;
   int4 next;
   auto describe = [&] {
     if (at == end) {
-      uint32_t x = __shfl_sync(0xffffffffu, ticket, 0);
+      if (!asked) ask();
+      asked = false;
+      const uint32_t x = __shfl_sync(0xffffffffu, ticket, 0);
       if (x >= taken) {
         // (every warp gets one that is too large: the last of them leaves the counter as it was found)
         if (taken && lane == 0 && x == taken + gridDim.x * S::kWarps - 1) *p.tickets = 0u;
@@ -217,7 +220,6 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
       member = x % p.side;
       at = cut.begin(run);
       end = cut.end(run);
-      take();
     }
     waiting = min(16, end - at);
     if (lane < waiting) {
@@ -441,8 +443,13 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
   int into = 0, from = 0;  // stages
 #pragma unroll 1
   for (int step = 0;; ++step) {
+    // (A run is taken no sooner than its first tile can follow the last one: one that is held back is one that no other
+    // warp takes.)
     if (waiting && made - used <= 16) store();
-    if (!waiting && !finished) describe();
+    if (!waiting && !finished) {
+      if (at < end || made - issued <= 1) describe();
+      else if (!asked && made - issued <= 2) ask();
+    }
     issue(into);
     into = into + 1 == S::kStages ? 0 : into + 1;
     if (step < S::kStages - 1) continue;
