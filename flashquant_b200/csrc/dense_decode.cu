@@ -153,6 +153,8 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
   const int g = lane >> 2, t = lane & 3;
   const int64_t room = int64_t(p.table_width) * p.block_size;
   const int unit_groups = p.hkv * p.chunks / p.side;
+  // (the wait first: the second kernel, which this lets start, reads what the kernels before this one have written)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // ---- the list: prefix sums of the sequences' tiles -------------------------------------------------
@@ -552,6 +554,7 @@ __global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const Dense
     o.w = fmaf(w, v.w, o.w);
   };
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   for (int i0 = 0; i0 < n; i0 += kJoinPieces) {
     const int some = min(kJoinPieces, n - i0);
     float4 ahead[kAhead];
@@ -654,6 +657,25 @@ static int dense_sms(int& sms) {
   return rc;
 }
 
+// Programmatic dependent launch: the kernel's CTAs may start while the one before it on the stream ends, and wait for it
+// themselves.
+static int launch_dependent(void (*kernel)(DenseArgs), const DenseArgs& p, dim3 grid, int threads, size_t smem,
+                            cudaStream_t stream) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, p);
+  if (e != cudaSuccess) return fail(FQ_ERR_CUDA, "dense decode: %s", cudaGetErrorString(e));
+  return check_launch("dense decode");
+}
+
 // As many heads to a CTA of the join as leave it with eight CTAs on an SM, all resident at once; where there are few
 // heads, their dimensions are split.
 template <typename T, int D>
@@ -667,18 +689,8 @@ static int launch_join(DenseArgs p, cudaStream_t stream) {
   while (p.join_rows < p.rows && 2 * p.join_rows <= kJoinRows && 2 * p.join_rows * p.join_wide / 4 <= kJoinThreads &&
          ctas() > most)
     p.join_rows *= 2;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(unsigned(units), (p.rows + p.join_rows - 1) / p.join_rows * (D / p.join_wide));
-  config.blockDim = dim3(kJoinThreads);
-  config.stream = stream;
-  cudaLaunchAttribute early;
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &early;
-  config.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&config, dense_join_kernel<T, D>, p);
-  if (e != cudaSuccess) return fail(FQ_ERR_CUDA, "dense decode: %s", cudaGetErrorString(e));
-  return check_launch("dense decode, join");
+  const unsigned parts = (p.rows + p.join_rows - 1) / p.join_rows * (D / p.join_wide);
+  return launch_dependent(dense_join_kernel<T, D>, p, dim3(unsigned(units), parts), kJoinThreads, 0, stream);
 }
 
 template <typename T, int D, bool R16>
@@ -697,8 +709,7 @@ static int launch_dense(const DenseArgs& p, int ctas, cudaStream_t stream) {
       return fail(FQ_ERR_CUDA, "dense decode: %s", cudaGetErrorString(e));
     }
   }
-  kernel<<<ctas, S::kWarps * 32, smem, stream>>>(p);
-  if (const int rc = check_launch("dense decode")) return rc;
+  if (const int rc = launch_dependent(kernel, p, dim3(ctas), S::kWarps * 32, smem, stream)) return rc;
   return launch_join<T, D>(p, stream);
 }
 template <typename T, int D>

@@ -45,7 +45,7 @@ FQ_HD DenseSpan dense_span(int len, int64_t room, int window) {
 constexpr int kDenseShare = 32;   // tiles of a share from which on there is a tail
 constexpr int kDenseMain = 13;    // entries of sixteen that are not in it
 constexpr int kDenseTaken = 8;    // runs taken per share, at most
-constexpr int kDenseShortest = 2; // tiles of a run at least, where there are enough
+constexpr int kDenseShortest = 1; // tiles of a run at least, where there are enough
 
 struct DenseCut {
   int total;                  // entries of the list (below 2^30)
