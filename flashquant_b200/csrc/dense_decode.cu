@@ -19,10 +19,14 @@
 // counter, 1 x 900 tokens took 20 us, and one warp had to read all pieces of a long sequence.
 #include <algorithm>
 
+#include <cooperative_groups.h>
+
 #include "dense_split.h"
 #include "fq_common.cuh"
 
 namespace fq {
+
+namespace cg = cooperative_groups;
 
 constexpr int kDenseMaxCtas = 148;
 constexpr int kDenseMaxSeqs = 2048;
@@ -469,10 +473,11 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
   cp_async_wait<0>();
 }
 
-// A CTA for `join_rows` query heads of a unit and `join_wide` of their dimensions: the weights of the pieces first, a warp
-// to a head and a lane to a piece, then the sums, a group of threads to a piece.  A unit that one run had is left alone;
-// heads without tokens get zeros.  What does not depend on the pieces is done before the wait for the first kernel, and
-// the first pieces are on their way with the weights.
+// A cluster for `join_rows` query heads of a unit and `join_wide` of their dimensions, each of its CTAs for a part of the
+// pieces: their weights first, a warp to a head and a lane to a piece, then the sums, a group of threads to a piece, and
+// the first CTA adds up what the others have in their shared memory.  A unit that one run had is left alone; heads without
+// tokens get zeros.  What does not depend on the pieces is done before the wait for the first kernel, and the first pieces
+// are on their way with the weights.  No CTA leaves before that wait: the kernel must not end before the first one has.
 constexpr int kJoinThreads = 128, kJoinPieces = 128, kJoinRows = 4;
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const DenseArgs p) {
@@ -481,6 +486,7 @@ __global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const Dense
   __shared__ float totals[kJoinRows][3];  // maximum, sum, factor of what stands
   __shared__ int counts[kWarps][2];
   __shared__ float4 sums[kJoinThreads];
+  const cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int units = p.hkv * p.chunks, unit_groups = units / p.side;
   const int seq = blockIdx.x / units, unit = blockIdx.x - seq * units;
@@ -488,7 +494,6 @@ __global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const Dense
   const DenseUnit u = dense_unit(p, unit);
   const int wides = D / p.join_wide, row0 = blockIdx.y / wides * p.join_rows;
   const int rows = min(p.join_rows, u.count - row0);
-  if (rows <= 0) return;
   const int columns = p.join_rows * p.join_wide / 4, groups = kJoinThreads / columns;  // float4
   const int mine = tid / columns, column = tid - mine * columns;
   const int row = column * 4 / p.join_wide;
@@ -529,17 +534,18 @@ __global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const Dense
     x.y = Dense16<T>::pack(o.z, o.w);
     *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (out_row + row) * D + dim) = x;
   };
-  const bool with_lse = p.lse && blockIdx.y % wides == 0;
-  if (tiles == 0) {
-    if (real && mine == 0) write(make_float4(0.f, 0.f, 0.f, 0.f));
-    if (with_lse && tid < rows) p.lse[out_row + tid] = -INFINITY;
-    return;
-  }
+  const bool with_lse = p.lse && blockIdx.y % wides == 0 && blockIdx.z == 0;
   const DenseCut cut = dense_cut(total, p.fixed);
   const int a = s0 + group * tiles;
   const DensePieces all = dense_pieces(cut, a, a + tiles);
-  const int n = all.count();
-  if (n == 1) return;
+  const int pieces = all.count(), first = pieces * blockIdx.z / gridDim.z, n = pieces * (blockIdx.z + 1) / gridDim.z;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tiles == 0 && blockIdx.z == 0) {
+    if (real && mine == 0) write(make_float4(0.f, 0.f, 0.f, 0.f));
+    if (with_lse && tid < rows) p.lse[out_row + tid] = -INFINITY;
+  }
+  if (tiles == 0 || pieces == 1 || rows <= 0) return;
   const int nth = seq * unit_groups + group, groups_all = p.seqs * unit_groups;
   auto piece = [&](int i) {
     return p.pieces + (int64_t(dense_slot(cut, all.run(i), nth, groups_all)) * p.side + member) * p.piece_floats;
@@ -553,9 +559,11 @@ __global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const Dense
     o.z = fmaf(w, v.z, o.z);
     o.w = fmaf(w, v.w, o.w);
   };
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  for (int i0 = 0; i0 < n; i0 += kJoinPieces) {
+  if (tid < kJoinRows) {
+    totals[tid][0] = -INFINITY;
+    totals[tid][1] = 0.f;
+  }
+  for (int i0 = first; i0 < n; i0 += kJoinPieces) {
     const int some = min(kJoinPieces, n - i0);
     float4 ahead[kAhead];
 #pragma unroll
@@ -563,7 +571,7 @@ __global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const Dense
       const int i = mine + k * groups;
       if (real && i < some) ahead[k] = *reinterpret_cast<const float4*>(piece(i0 + i) + offset);
     }
-    if (i0) __syncthreads();  // the weights before have been used
+    __syncthreads();  // the weights before have been used
     if (warp < rows) {
       float2 x[kJoinPieces / 32];
       float now = m;
@@ -608,11 +616,29 @@ __global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const Dense
   }
   sums[tid] = o;
   __syncthreads();
-  if (with_lse && tid < rows) p.lse[out_row + tid] = dense_lse(totals[tid][0], totals[tid][1], Dense16<T>::kLift);
-  if (!real || mine > 0) return;
-  for (int i = 1; i < groups; ++i) add(1.f, sums[i * columns + column]);
-  const float sum = totals[row][1], f = sum == 0.f ? 0.f : 1.f / sum;
-  write(make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+  if (real && mine == 0) {
+    for (int i = 1; i < groups; ++i) add(1.f, sums[i * columns + column]);
+    sums[tid] = o;
+  }
+  if (gridDim.z > 1) cluster.sync();
+  if (blockIdx.z == 0) {
+    float top = -INFINITY, sum = 0.f;  // of all CTAs, of the thread's row
+    if (real && mine == 0) {
+      for (unsigned z = 0; z < gridDim.z; ++z) top = fmaxf(top, cluster.map_shared_rank(&totals[row][0], z)[0]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (unsigned z = 0; z < gridDim.z; ++z) {
+        const float* of = cluster.map_shared_rank(&totals[row][0], z);
+        const float w = fast_exp2(of[0] - ref);
+        sum = fmaf(w, of[1], sum);
+        add(w, *cluster.map_shared_rank(&sums[tid], z));
+      }
+      const float f = sum == 0.f ? 0.f : 1.f / sum;
+      write(make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+      if (with_lse && column * 4 == row * p.join_wide) p.lse[out_row + row] = dense_lse(top, sum, Dense16<T>::kLift);
+    }
+  }
+  if (gridDim.z > 1) cluster.sync();  // what the first CTA reads stays
 }
 
 // ------------------------------------------------------------------------------------
@@ -666,18 +692,22 @@ static int launch_dependent(void (*kernel)(DenseArgs), const DenseArgs& p, dim3 
   config.blockDim = dim3(threads);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
-  cudaLaunchAttribute early;
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &early;
-  config.numAttrs = 1;
+  cudaLaunchAttribute attributes[2];
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;  // the CTAs along z
+  attributes[1].val.clusterDim.x = attributes[1].val.clusterDim.y = 1;
+  attributes[1].val.clusterDim.z = grid.z;
+  config.attrs = attributes;
+  config.numAttrs = grid.z > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&config, kernel, p);
   if (e != cudaSuccess) return fail(FQ_ERR_CUDA, "dense decode: %s", cudaGetErrorString(e));
   return check_launch("dense decode");
 }
 
 // As many heads to a CTA of the join as leave it with eight CTAs on an SM, all resident at once; where there are few
-// heads, their dimensions are split.
+// heads, their dimensions are split, and the pieces of a unit where it can have hundreds (1 x 131072 tokens, 8 query
+// heads on one KV head: 55 us without, ... with).
 template <typename T, int D>
 static int launch_join(DenseArgs p, cudaStream_t stream) {
   const int64_t units = int64_t(p.seqs) * p.hkv * p.chunks, most = 8 * kDenseMaxCtas;
@@ -690,7 +720,11 @@ static int launch_join(DenseArgs p, cudaStream_t stream) {
          ctas() > most)
     p.join_rows *= 2;
   const unsigned parts = (p.rows + p.join_rows - 1) / p.join_rows * (D / p.join_wide);
-  return launch_dependent(dense_join_kernel<T, D>, p, dim3(unsigned(units), parts), kJoinThreads, 0, stream);
+  const int64_t tiles = int64_t(p.table_width) * (p.block_size / kDenseTile);
+  const int64_t pieces = std::min(tiles, int64_t(p.fixed) * (1 + kDenseTaken) * p.side / units);  // of a unit, about
+  unsigned split = 1;
+  while (split < 8 && pieces > 64 * split && 2 * split * ctas() <= most) split *= 2;
+  return launch_dependent(dense_join_kernel<T, D>, p, dim3(unsigned(units), parts, split), kJoinThreads, 0, stream);
 }
 
 template <typename T, int D, bool R16>
