@@ -449,10 +449,11 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
   int into = 0, from = 0;  // stages
 #pragma unroll 1
   for (int step = 0;; ++step) {
-    // (A run is taken no sooner than its first tile can follow the last one: one that is held back is one that no other
-    // warp takes.)
-    if (waiting && made - used <= 16) store();
-    if (!waiting && !finished) {
+    // The next tiles are described when eight are left, and stored, with their pages' ids, when four are.  A run is taken
+    // no sooner than its first tile can follow the last one: one that is held back is one that no other warp takes.
+    if (waiting) {
+      if (made - issued <= 4) store();
+    } else if (!finished && made - issued <= 8) {
       if (at < end || made - issued <= 1) describe();
       else if (!asked && made - issued <= 2) ask();
     }

@@ -5,12 +5,11 @@
 // of a sequence stand side by side (they are given to warps that run at the same time, so that the heads of a
 // token, which are adjacent in a page, are read together).  The tiles of 16 tokens of all unit groups of all
 // sequences form one list of `total` entries, cut into runs whatever the bounds between sequences are: a ragged
-// batch is balanced.  Where a warp's share is long enough, thirteen of every sixteen entries are dealt out beforehand
-// and the other three ("tail") in runs of a sixteenth, then a forty-eighth, of a share that warps take when they are
-// free: SMs do not get the same share of the memory's bandwidth (8 sequences of 32k - 131k tokens, equal runs: the
-// first SM was through after 345 us, the last after 483).  Every sequence has its part of the tail, since many short
-// runs are many pieces to join (with the tail at the list's end its last two sequences had 800 each, which took 14 us
-// where the others took 3).  Where the cuts are never depends on who takes a run.
+// batch is balanced.  Where a warp's share is long, some of every sixteen entries (the "tail") are not dealt out
+// beforehand but in short runs that warps take when they are free: SMs do not get the same share of the memory's
+// bandwidth (8 sequences of 32k - 131k tokens, equal runs: the first warp was through after 350 us, the last after 456).
+// Every sequence has its part of the tail, since short runs are pieces to join.  Where the cuts are never depends on
+// who takes a run.
 #pragma once
 
 #include <stdint.h>
@@ -42,19 +41,20 @@ FQ_HD DenseSpan dense_span(int len, int64_t room, int window) {
   return s;
 }
 
-constexpr int kDenseShare = 32;   // tiles of a share from which on there is a tail
-constexpr int kDenseMain = 13;    // entries of sixteen that are not in it
-constexpr int kDenseTaken = 8;    // runs taken per share, at most
-constexpr int kDenseShortest = 1; // tiles of a run at least, where there are enough
+// Tiles of a share from which on there is a tail.  Queries, pieces and their join cost more than the balance gives below:
+// 32 x 4096 tokens (a share of 55) 92 us without, 92 - 100 with one; 64 x 2000, head_dim 256 (108) 198, 211 - 219; ragged
+// 8 x 131072 (300) 445 and, after other data, 500 without, 428 and 475 with one.
+constexpr int kDenseShare = 192;
+constexpr int kDenseMain = 14;    // entries of sixteen that are not in the tail
+constexpr int kDenseTaken = 4;    // runs taken per share, at most
+constexpr int kDenseShortest = 1; // tiles of a run at least
 
 struct DenseCut {
   int total;                  // entries of the list (below 2^30)
   bool split;                 // there is a tail
   int fixed;                  // runs that are dealt out beforehand, of the others
   int mains, length;          // entries of these, of one of them
-  int tails;                  // entries of the tail
-  int medium, length2, bound; // runs of the tail's first `bound` entries, their length
-  int length3;                // of a run behind
+  int tails, shorter;         // entries of the tail, of one of its runs
 
   // entries of the main kind before entry x of the list, and back from either kind
   FQ_HD int main_of(int x) const {
@@ -67,23 +67,18 @@ struct DenseCut {
   }
   // runs count through; the entries of a run are of its own kind
   FQ_HD bool is_tail(int run) const { return run >= fixed; }
-  FQ_HD int run_of(bool tail, int i) const {
-    return !tail ? i / length : (i < bound ? fixed + i / length2 : fixed + medium + (i - bound) / length3);
-  }
+  FQ_HD int run_of(bool tail, int i) const { return tail ? fixed + i / shorter : i / length; }
   FQ_HD int begin(int run) const {
-    if (run < fixed) {
-      const int64_t x = int64_t(run) * length;
-      return x < mains ? int(x) : mains;
-    }
-    const int64_t x = run < fixed + medium ? int64_t(run - fixed) * length2 : bound + int64_t(run - fixed - medium) * length3;
-    return x < tails ? int(x) : tails;
-  }
-  FQ_HD int end(int run) const {
-    const int64_t x = int64_t(begin(run)) + (run < fixed ? length : (run < fixed + medium ? length2 : length3));
-    const int most = run < fixed ? mains : tails;
+    const int64_t x = is_tail(run) ? int64_t(run - fixed) * shorter : int64_t(run) * length;
+    const int most = is_tail(run) ? tails : mains;
     return x < most ? int(x) : most;
   }
-  FQ_HD int taken() const { return split ? medium + (tails - bound + length3 - 1) / length3 : 0; }
+  FQ_HD int end(int run) const {
+    const int64_t x = int64_t(begin(run)) + (is_tail(run) ? shorter : length);
+    const int most = is_tail(run) ? tails : mains;
+    return x < most ? int(x) : most;
+  }
+  FQ_HD int taken() const { return (tails + shorter - 1) / shorter; }
 };
 FQ_HD DenseCut dense_cut(int total, int fixed) {
   DenseCut c;
@@ -95,10 +90,7 @@ FQ_HD DenseCut dense_cut(int total, int fixed) {
   c.tails = total - c.mains;
   c.length = c.split ? (c.mains + fixed - 1) / fixed : share;
   if (c.length < kDenseShortest) c.length = kDenseShortest;
-  c.length2 = (share + 15) / 16;
-  c.length3 = share < 96 ? 2 : (share + 47) / 48;
-  c.medium = c.tails < fixed * c.length2 ? c.tails / c.length2 : fixed;
-  c.bound = c.medium * c.length2;
+  c.shorter = share / 24 + 1;
   return c;
 }
 

@@ -204,7 +204,7 @@ def test_decode_refusals(kw, rc):
 
 def test_decode_workspace_sizes():
     f = N.load().fq_dense_paged_decode_workspace_bytes
-    assert f(4, 32, 8, 128) >= 32768 + 148 * 9 * 8 * 4 * 130 * 4
+    assert f(4, 32, 8, 128) >= 32768 + 148 * 5 * 8 * 4 * 130 * 4
     assert f(4, 32, 8, 80) == 0 and f(4, 12, 8, 128) == 0 and f(-1, 8, 8, 128) == 0
     assert f(1, 32, 8, 128) < f(2048, 32, 8, 128)
 
