@@ -621,7 +621,7 @@ __global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const Dense
     for (int i = 1; i < groups; ++i) add(1.f, sums[i * columns + column]);
     sums[tid] = o;
   }
-  if (gridDim.z > 1) cluster.sync();
+  if (gridDim.z > 1) cluster_barrier();
   if (blockIdx.z == 0) {
     float top = -INFINITY, sum = 0.f;  // of all CTAs, of the thread's row
     if (real && mine == 0) {
@@ -639,7 +639,7 @@ __global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const Dense
       if (with_lse && column * 4 == row * p.join_wide) p.lse[out_row + row] = dense_lse(top, sum, Dense16<T>::kLift);
     }
   }
-  if (gridDim.z > 1) cluster.sync();  // what the first CTA reads stays
+  if (gridDim.z > 1) cluster_barrier();  // what the first CTA reads stays
 }
 
 // ------------------------------------------------------------------------------------

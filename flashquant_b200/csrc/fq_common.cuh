@@ -266,6 +266,13 @@ __device__ __forceinline__ void bulk_g2s_hint(void* smem_dst, const void* gmem_s
       : "memory");
 }
 
+// A barrier of all threads of a cluster (of the CTA, where it is launched without one); what was written before it is
+// visible behind it.  The form that does not ask for converged warps: it stands behind branches that only some lanes take.
+__device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
 // Orders this thread's earlier generic-proxy accesses (and those it has acquired from other
 // threads) before its later bulk copies, which go through the async proxy.
 __device__ __forceinline__ void fence_proxy_async() {

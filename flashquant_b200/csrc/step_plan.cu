@@ -8,13 +8,9 @@
 // for.
 #include <algorithm>
 
-#include <cooperative_groups.h>
-
 #include "fq_common.cuh"
 
 namespace fq {
-
-namespace cg = cooperative_groups;
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanBatch = 4;  // pages or tokens of a thread whose loads are in flight together
@@ -223,7 +219,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(const PlanArgs 
       p.positions[x] = at[k];
     }
   }
-  cg::this_cluster().sync();  // (of one CTA, unless free_count is count_out)
+  cluster_barrier();  // (of one CTA, unless free_count is count_out)
   if (cta == 0 && tid == 0) *p.count_out = int32_t(height - all_pages);
 }
 
@@ -283,7 +279,7 @@ __global__ void __launch_bounds__(kPlanThreads) release_pages_kernel(const Relea
       if (x < total) p.free_pages[height + x] = id[k];
     }
   }
-  cg::this_cluster().sync();
+  cluster_barrier();
   if (cta == 0 && tid == 0) *p.count_out = int32_t(height + total);
 }
 
