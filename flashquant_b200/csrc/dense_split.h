@@ -37,7 +37,7 @@ FQ_HD DenseSpan dense_span(int len, int64_t room, int window) {
   s.len = len < 0 ? 0 : (len > room ? int(room) : len);
   s.begin = window > 0 && window < s.len ? s.len - window : 0;
   s.first_tile = s.begin / kDenseTile;
-  s.tiles = (s.len + kDenseTile - 1) / kDenseTile - s.first_tile;
+  s.tiles = s.len > 0 ? (s.len - 1) / kDenseTile + 1 - s.first_tile : 0;
   return s;
 }
 

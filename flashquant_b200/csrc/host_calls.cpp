@@ -695,7 +695,6 @@ PyObject* dense_decode(PyObject*, Args a, Py_ssize_t n) {
     return none();
   Tensor out, lse;
   if (!decode_out(a[7], *q, dev, out)) return none();
-  if (a[7] == Py_None && !out.is_contiguous()) out = at::empty(q->sizes(), q->options());
   if (a[8] == Py_True) lse = at::empty({seqs, hq}, q->options().dtype(at::kFloat));
   const int hkv = int(kc->size(2));
   const size_t need = std::max<size_t>(fq_dense_paged_decode_workspace_bytes(int(seqs), int(hq), hkv, int(d)), 32768);

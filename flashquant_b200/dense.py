@@ -281,8 +281,9 @@ def rotary_append_dense(q, key, value, key_cache, value_cache, slot_mapping, pos
     launch.  Returns the rotated ``q`` (``q_out``, which may be ``q``); None if ``q`` is None.
 
     Without ``positions`` and ``frequencies`` nothing is rotated (and ``q`` must be None).  A slot is
-    ``block * block_size + token``, as in ``tq4_compress_append``; negative ones are skipped.  The queries of
-    such a token are still rotated if its position is not negative, its keys are stored only if it is not.
+    ``block * block_size + token``, as in ``tq4_compress_append``; negative ones, and those beyond the pages, are
+    skipped, the others are distinct.  A token with a negative position has its values stored, not its queries
+    and keys.
     """
     code = _layout(layout)
     r = _host().rotary_append_dense(q, key, value, key_cache, value_cache, slot_mapping, positions, frequencies,

@@ -613,7 +613,8 @@ int fq_decode_step_host_packed(const void* block_host, void* out_host, int overl
  * new tokens (-1 behind the last), served (1 byte a request), *free_count_out (may be free_count).
  * A request is served if the stack holds the pages, and slot_mapping the tokens, of all requests up
  * to and including it; one without new tokens always is.  A negative length, or more pages than a
- * row holds, is not served and takes nothing.  At most 4096 requests.
+ * row holds, is not served and takes nothing.  At most 4096 requests; the outputs, but for
+ * *free_count_out, share no memory with the inputs.
  */
 int fq_plan_paged_step(const int32_t* context_lens, const int32_t* query_lens, int num_requests,
                        int32_t* block_table, int64_t block_table_stride, int block_table_width,
@@ -658,7 +659,8 @@ int fq_rotary_embed(const void* q, const void* k, fq_dtype dtype, int64_t tokens
  * value_cache.  A slot outside [0, num_slots) stores nothing; rotary_dim = 0 appends as it is.
  *   strides        q token, q head, key token, key head, value token, value head, q_out token,
  *                  q_out head, then block, token, head of key_cache and of value_cache
- * A slot is block * block_size + token, as in fq_tq4_compress_append.
+ * A slot is block * block_size + token, as in fq_tq4_compress_append; the slots of a call are
+ * distinct.  q_out may be q.
  */
 int fq_rotary_append_dense(const void* q, const void* key, const void* value, fq_dtype dtype,
                            int64_t tokens, int num_q_heads, int num_kv_heads, int head_dim,
@@ -671,7 +673,7 @@ int fq_rotary_append_dense(const void* q, const void* key, const void* value, fq
 /*
  * Attention of one query token per sequence over pages of 16-bit keys and values: the layers of a
  * model whose cache is not compressed, over the block tables of those that are
- * (fq_split_k_paged_decode).  One launch, split over the tokens and joined in it.
+ * (fq_split_k_paged_decode).  Split over the tokens; the parts are joined by a second kernel.
  *   q              (num_seqs, num_q_heads, head_dim), strides in elements
  *   key_cache,     row (block, token, head) at block * *_block_stride + token * *_token_stride +
  *   value_cache    head * *_head_stride; rows start at multiples of 16 bytes

@@ -76,6 +76,13 @@ int main() {
     int a = 0, b = 0;
     CHECK(c.taken() == 0 && c.begin(0) == 0 && c.end(0) == 0 && c.end(147) == 0);
   }
+  {
+    const DenseSpan s = dense_span(2147483647, int64_t(1) << 33, 0), w = dense_span(2147483647, int64_t(1) << 33, 5);
+    const DenseCut c = dense_cut(1, 1);
+    int a = 0, b = 0;
+    CHECK(s.len == 2147483647 && s.tiles == 1 << 27 && s.first_tile == 0);
+    CHECK(w.begin == 2147483642 && w.first_tile == (1 << 27) - 1 && w.tiles == 1);
+  }
   for (int len = -3; len < 200; ++len)
     for (int window = 0; window < 70; ++window)
       for (int room = 0; room <= 160; room += 16) {

@@ -14,6 +14,7 @@ Tolerances are sums of what each rounding may do, at most; u = 2^-24 is half a s
 
 import math
 import random
+import threading
 
 import pytest
 import torch
@@ -237,6 +238,22 @@ def test_decode_repeats_bit_for_bit():
     assert all(torch.equal(c.call(), want) for _ in range(50))
 
 
+@pytest.mark.parametrize("hq, hkv, d, lens, window", [
+    (32, 8, 128, [230001, 3, 131072, 0, 77000, 60123], 0), (8, 1, 128, [1500000, 17, 2300000], 0),
+    (16, 16, 64, [300000, 1, 180007, 90000], 0), (20, 2, 256, [70000, 500000, 16, 430000], 0),
+    (32, 8, 128, [400000, 5, 390007], 300000)])
+def test_decode_long_lists(hq, hkv, d, lens, window):
+    """Lists of which warps take a part when they are free (1.9 GB of keys and values): right, and the same bits
+    whoever takes what; the workspace's head is left as it was."""
+    b = Batch(lens, hq, hkv, d, BF, block=64, window=window)
+    ws = torch.zeros(N.load().fq_dense_paged_decode_workspace_bytes(len(lens), hq, hkv, d), dtype=torch.uint8, device=DEV)
+    out, lse = b.call(return_lse=True, workspace=ws)
+    b.check(out, lse)
+    for _ in range(15):
+        assert torch.equal(b.call(workspace=ws), out)
+    assert not ws[:32768].any()
+
+
 def test_decode_on_two_streams():
     a, b = Batch([4000, 9, 1300], 32, 8, 128, BF), Batch([2, 5000], 8, 1, 64, HF, seed=5)
     want = a.call(), b.call()
@@ -280,6 +297,77 @@ def test_two_recorded_decodes_side_by_side():
     assert not outs[0].any()
     for graph in graphs:
         graph.reset()
+
+
+def test_what_follows_waits_for_all_of_a_decode():
+    """A batch of which no unit has to be joined, long enough to be under way when what follows it is launched:
+    eager and recorded, the reader of its output sees all of it."""
+    b = Batch([16000] * 4 + [1] * 400, 64, 8, 128, BF)
+    b.table[:4] = b.table[:1]  # (the long ones share pages)
+    b.rows[:4] = [b.rows[0]] * 4
+    want = b.call()
+    b.check(want, only=[0, 3, 4, 403])
+    short = Batch([300] * 200, 16, 16, 64, HF)
+    want_short = short.call()
+    out, copy = torch.empty_like(want_short), torch.empty_like(want_short)
+    for _ in range(30):
+        out.fill_(float("nan"))
+        short.call(out=out)
+        copy.copy_(out)
+        assert torch.equal(copy, want_short)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for x, y in ((short, out),):
+            y.fill_(float("nan"))
+            x.call(out=y)
+            copy.copy_(y)
+            first = b.call()
+            second = first + 0
+    for _ in range(20):
+        copy.zero_(), second.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(copy, want_short) and torch.equal(second, want)
+    graph.reset()
+
+
+def test_decodes_from_two_threads_on_one_stream():
+    a, b = Batch([4000, 9, 1300], 32, 8, 128, BF), Batch([2, 5000, 77], 32, 8, 128, BF, seed=5)
+    want = a.call(), b.call()
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(x, w):
+        outs = [x.call() for _ in range(60)]
+        torch.cuda.synchronize()
+        wrong.extend(o for o in outs if not torch.equal(o, w))
+    threads = [threading.Thread(target=work, args=z) for z in zip((a, b), want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_calls_without_anything_to_do():
+    none = torch.zeros(0, dtype=torch.int32, device=DEV)
+    pages = torch.zeros(2, 16, 8, 128, dtype=BF, device=DEV)
+    q = torch.zeros(0, 32, 128, dtype=BF, device=DEV)
+    out, lse = fq.split_k_paged_decode_dense(q, pages, pages, none.view(0, 4), none, return_lse=True)
+    assert out.shape == (0, 32, 128) and lse.shape == (0, 32)
+    freq, _ = fq.rotary_frequencies(128, device=DEV)
+    kv = torch.zeros(0, 8, 128, dtype=BF, device=DEV)
+    assert [x.shape[0] for x in fq.rotary_embed(q, kv, none, freq)] == [0, 0]
+    assert fq.rotary_append_dense(q, kv, kv, pages, pages, none, none, freq).shape == (0, 32, 128)
+    q = torch.randn(3, 32, 128, device=DEV).to(BF)  # a block table without columns: no tokens
+    zero = torch.zeros(3, dtype=torch.int32, device=DEV)
+    assert not fq.split_k_paged_decode_dense(q, pages, pages, none.view(3, 0), zero).any()
+    heads = torch.zeros(4, 0, 128, dtype=BF, device=DEV)
+    x, y = fq.rotary_embed(heads, heads, torch.arange(4, device=DEV), freq)
+    assert x.shape == y.shape == (4, 0, 128)
+    room = fq.plan_paged_step(none, none, none.view(0, 4), none, zero[:1], 16, 0)
+    assert room.cu_seqlens_q.tolist() == [0] and room.slot_mapping.numel() == 0 and int(room.free_count) == 0
+    assert int(fq.release_pages(none.bool(), none, none.view(0, 4), none, zero[:1], 16)) == 0
 
 
 def test_decode_through_ctypes_alone(monkeypatch):
