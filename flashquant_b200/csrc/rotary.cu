@@ -61,10 +61,14 @@ struct RotaryJobs {
       : places(all < 32 ? all : 32), side(32 / places), parts((all + 31) / 32),
         count((heads + rows * side - 1) / (rows * side) * parts) {}
 };
-// Places of a row of q or k (v: without a part that is turned), the values of a place in one vector or in two.
+// The values of a place stand in one vector or in two: of a part that is turned the two of its pairs, of one that is kept
+// two that are half of it apart.  Places of a part of `values`:
 __host__ __device__ inline bool rotary_two(int n, bool half_layout) { return half_layout || n == 1; }
+__host__ __device__ inline int rotary_kept(int n, bool half_layout, int values) {
+  return values / (rotary_two(n, half_layout) && values % (2 * n) == 0 ? 2 * n : n);
+}
 __host__ __device__ inline int rotary_places(int n, bool half_layout, int head_dim, int rotary_dim) {
-  return rotary_dim / (rotary_two(n, half_layout) ? 2 * n : n) + (head_dim - rotary_dim) / n;
+  return rotary_dim / (rotary_two(n, half_layout) ? 2 * n : n) + rotary_kept(n, half_layout, head_dim - rotary_dim);
 }
 __host__ __device__ inline int rotary_rows(int n, bool half_layout) { return rotary_two(n, half_layout) ? 2 : 4; }
 
@@ -89,7 +93,7 @@ __device__ __forceinline__ void put2(__nv_bfloat16* at, float x, float y) {
 
 // N values to a vector.  HALF: pairs half a rotated part apart, else adjacent.
 template <typename T, int N, bool HALF>
-__global__ void __launch_bounds__(kRotWarps * 32, 3) rotary_kernel(const RotaryArgs p, int batch) {
+__global__ void __launch_bounds__(kRotWarps * 32, 4) rotary_kernel(const RotaryArgs p, int batch) {
   using V = Vec<T, N>;
   constexpr int kPairs = HALF ? N : (N > 1 ? N / 2 : 1), kRows = HALF || N == 1 ? 2 : 4;
   constexpr bool kTwo = HALF || N == 1;  // the values of a place stand in two vectors
@@ -128,8 +132,7 @@ __global__ void __launch_bounds__(kRotWarps * 32, 3) rotary_kernel(const RotaryA
 
   // ---- this warp's job ---------------------------------------------------------------------------------
   const int all = rotary_places(N, HALF, p.head_dim, p.rotary_dim);
-  const bool halves = kTwo && p.head_dim % (2 * N) == 0;  // of a row of v, copied by places like those that are turned
-  const int all_v = p.head_dim / (halves ? 2 * N : N);
+  const int all_v = rotary_kept(N, HALF, p.head_dim);
   const RotaryJobs jq(all, p.q.heads, kRows), jk(all, p.k.heads, kRows), jv(all_v, p.v.heads, kRows);
   int job = blockIdx.y * (blockDim.x / 32) + __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int kind = job < jq.count ? 0 : (job < jq.count + jk.count ? 1 : 2);
@@ -141,15 +144,15 @@ __global__ void __launch_bounds__(kRotWarps * 32, 3) rotary_kernel(const RotaryA
   const int row = lane / j.places, place = job % j.parts * 32 + lane - row * j.places;
   const int head = job / j.parts * kRows * j.side + row;
   const bool turned = kind < 2 && place < turns_of;
-  const bool two = kind == 2 ? halves : kTwo && turned;
+  const int kept = kind == 2 ? p.head_dim : p.head_dim - p.rotary_dim;
+  const bool two = kTwo && (turned || kept % (2 * N) == 0);
   const int rows = !working || row >= j.side || place >= (kind == 2 ? all_v : all) || head >= t.heads
                        ? 0
                        : min(kRows, (t.heads - head + j.side - 1) / j.side);
   int at = place * N, too = 0;  // the values of a place; how far its second vector is behind the first
-  if (kind == 2) {
-    too = p.head_dim / 2;
-  } else if (!turned) {
-    at = p.rotary_dim + (place - turns_of) * N;
+  if (!turned) {
+    if (kind < 2) at += p.rotary_dim - turns_of * N;
+    too = kept / 2;
   } else if (kTwo) {
     if (!HALF) at = 2 * place;
     too = HALF ? half : 1;
@@ -248,7 +251,7 @@ static int launch_rotary(const RotaryArgs& p, bool half_layout, cudaStream_t str
                     p.head_dim % N == 0 && p.rotary_dim % (half_layout ? 2 * N : N) == 0;
   const int n = wide ? N : 1, rows = rotary_rows(n, half_layout);
   const int all = rotary_places(n, half_layout, p.head_dim, p.rotary_dim);
-  const int all_v = p.head_dim / (rotary_two(n, half_layout) && p.head_dim % (2 * n) == 0 ? 2 * n : n);
+  const int all_v = rotary_kept(n, half_layout, p.head_dim);
   const int jobs = RotaryJobs(all, p.q.heads, rows).count + RotaryJobs(all, p.k.heads, rows).count +
                    RotaryJobs(all_v, p.v.heads, rows).count;
   const int groups = (jobs + kRotWarps - 1) / kRotWarps, warps = (jobs + groups - 1) / groups;
