@@ -807,8 +807,8 @@ extern "C" int fq_dense_paged_decode(
   FQ_REQUIRE(aligned(key_cache, 16) && aligned(value_cache, 16) && (k_block_stride | k_token_stride | k_head_stride |
              v_block_stride | v_token_stride | v_head_stride) % 8 == 0, FQ_ERR_ALIGNMENT,
              "dense decode: rows of the caches must start at multiples of 16 bytes");
-  FQ_REQUIRE(aligned(q, 4) && (q_seq_stride | q_head_stride) % 2 == 0 && aligned(out, 4), FQ_ERR_ALIGNMENT,
-             "dense decode: rows of q and out must start at multiples of 4 bytes");
+  FQ_REQUIRE(aligned(q, 4) && (q_seq_stride | q_head_stride) % 2 == 0 && aligned(out, 8), FQ_ERR_ALIGNMENT,
+             "dense decode: rows of q must start at multiples of 4 bytes, out at one of 8");
   const DenseGeometry x = dense_geometry(num_q_heads, num_kv_heads, head_dim);
   const int64_t unit_groups = int64_t(num_kv_heads) * x.chunks / x.side;
   const int64_t most = num_seqs * unit_groups * block_table_width * (block_size / kDenseTile);

@@ -561,11 +561,18 @@ const Tensor* rows(PyObject* o, int dev) {
   const Tensor* t = on_device(o, dev);
   return t && t->dim() == 3 && t->stride(2) == 1 ? t : nullptr;
 }
-// no two rows share memory
+// no two rows (of the last dimension) share memory
 bool own_rows(const Tensor& t) {
-  const int64_t n = t.size(0), h = t.size(1), d = t.size(2), s = t.stride(0), u = t.stride(1);
-  return ((h == 1 || u >= d) && (n == 1 || s >= (h - 1) * u + d)) ||
-         ((n == 1 || s >= d) && (h == 1 || u >= (n - 1) * s + d));
+  int order[3], n = 0;  // the other dimensions by their strides
+  for (int i = 0; i + 1 < t.dim() && n < 3; ++i)
+    if (t.size(i) > 1) order[n++] = i;
+  std::sort(order, order + n, [&](int i, int j) { return t.stride(i) < t.stride(j); });
+  int64_t extent = t.size(-1);
+  for (int k = 0; k < n; ++k) {
+    if (t.stride(order[k]) < extent) return false;
+    extent += t.stride(order[k]) * (t.size(order[k]) - 1);
+  }
+  return true;
 }
 // None makes a new tensor
 bool out_rows(PyObject* o, const Tensor& like, int dev, Tensor& out) {
@@ -582,9 +589,7 @@ bool out_rows(PyObject* o, const Tensor& like, int dev, Tensor& out) {
 const Tensor* pages(PyObject* o, int dev, at::ScalarType st, bool written) {
   const Tensor* t = on_device(o, dev);
   if (!t || t->dim() != 4 || t->scalar_type() != st || t->stride(3) != 1) return nullptr;
-  for (int i = 0; written && i < 3; ++i)
-    if (t->size(i) > 1 && t->stride(i) < t->size(3)) return nullptr;
-  return t;
+  return written && !own_rows(*t) ? nullptr : t;
 }
 const Tensor* ints(PyObject* o, int dev, int64_t n) {
   const Tensor* t = dense(o, dev);

@@ -190,16 +190,17 @@ def _rows(t, name, tokens=None, dtype=None):
 
 
 def _own_rows(t) -> bool:
-    """No two rows of ``t`` (tokens, heads, D) share memory."""
-    n, h, d = t.shape
-    s, u = t.stride(0), t.stride(1)
-    if n == 0 or h == 0 or d == 0:
+    """No two rows (of the last dimension) of ``t`` share memory."""
+    if t.numel() == 0:
         return True
-    if d > 1 and t.stride(2) != 1:
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
         return False
-    by_token = (h == 1 or u >= d) and (n == 1 or s >= (h - 1) * u + d)
-    by_head = (n == 1 or s >= d) and (h == 1 or u >= (n - 1) * s + d)
-    return by_token or by_head
+    extent = t.shape[-1]
+    for s, n in sorted((s, n) for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+        if s < extent:
+            return False
+        extent += s * (n - 1)
+    return True
 
 
 def _rotary_args(head_dim, tokens, positions, frequencies, dev):
@@ -266,9 +267,7 @@ def rotary_embed(q, k, positions, frequencies, *, layout: str = "half", scale: f
 
 
 def _cache(t, name, like):
-    if t.dim() != 4 or t.dtype != like.dtype or t.device != like.device or \
-            (t.shape[3] > 1 and t.stride(3) != 1) or any(n > 1 and s < t.shape[3] for n, s in
-                                                         zip(t.shape[:3], t.stride()[:3])):
+    if t.dim() != 4 or t.dtype != like.dtype or t.device != like.device or not _own_rows(t):
         raise ValueError(f"{name} must be (num_blocks, block_size, H_kv, D) of the type of the others, "
                          "rows of adjacent values that are its own")
     return t

@@ -678,7 +678,7 @@ int fq_rotary_append_dense(const void* q, const void* key, const void* value, fq
  *   key_cache,     row (block, token, head) at block * *_block_stride + token * *_token_stride +
  *   value_cache    head * *_head_stride; rows start at multiples of 16 bytes
  *   window         each sequence sees its last `window` tokens (0: all)
- *   out            contiguous like q; zeros for a sequence without tokens
+ *   out            contiguous, 8-byte aligned; zeros for a sequence without tokens
  *   lse            optional (num_seqs, num_q_heads): the natural logarithm of the sum of
  *                  exp(sm_scale q k); -inf without tokens
  *   workspace      fq_dense_paged_decode_workspace_bytes(...), 16-byte aligned, one per

@@ -179,7 +179,9 @@ def test_there_is_no_cpu_path():
                                                ((0, 128, 1), (3, 2, 128), False), ((128, 128, 1), (3, 2, 128), False),
                                                ((256, 0, 1), (3, 2, 128), False), ((256, 64, 1), (3, 2, 128), False),
                                                ((7, 7, 1), (1, 1, 128), True), ((0, 0, 1), (0, 2, 128), True),
-                                               ((256, 128, 2), (3, 2, 128), False)])
+                                               ((256, 128, 2), (3, 2, 128), False), ((1024, 64, 64, 1), (2, 4, 4, 64), False),
+                                               ((1024, 256, 64, 1), (2, 4, 4, 64), True), ((1024, 64, 256, 1), (2, 4, 4, 64), True),
+                                               ((960, 256, 64, 1), (2, 4, 4, 64), False)])
 def test_rows_of_their_own(stride, size, own):
     assert dense._own_rows(torch.empty_strided(size, stride)) is own
 
@@ -201,7 +203,7 @@ def _decode(**kw):
                                     (dict(hq=12), -1), (dict(hkv=0), -1), (dict(d=80), -2), (dict(seqs=2049), -2),
                                     (dict(bs=24), -2), (dict(bs=0), -2), (dict(dtype=N.FQ_F32), -2),
                                     (dict(kt=1020), -5), (dict(vh=4), -5), (dict(k=ctypes.c_void_p(4104)), -5),
-                                    (dict(q=ctypes.c_void_p(4098)), -5), (dict(qs=1023), -5), (dict(ws=None), -3),
+                                    (dict(q=ctypes.c_void_p(4098)), -5), (dict(qs=1023), -5), (dict(out=ctypes.c_void_p(4100)), -5), (dict(ws=None), -3),
                                     (dict(bytes=32768), -3), (dict(width=1 << 29), -2), (dict(seqs=0, q=None), 0)])
 def test_decode_refusals(kw, rc):
     assert _decode(**kw) == rc

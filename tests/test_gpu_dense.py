@@ -186,6 +186,7 @@ def test_decode_refusals():
     refused(window=-1)
     refused(out=torch.empty(2, 32, 64, dtype=BF, device=DEV))
     refused(N.FlashQuantNativeError, workspace=torch.zeros(1024, dtype=torch.uint8, device=DEV))
+    refused(N.FlashQuantNativeError, out=torch.zeros(2 * 32 * 128 + 2, dtype=BF, device=DEV)[2:].view(2, 32, 128))
     refused(N.FlashQuantNativeError, q=torch.zeros(2, 12, 128, dtype=BF, device=DEV))
     refused(N.FlashQuantNativeError, seq_lens=b.sl.cpu())
     odd = torch.zeros(8 * 16 * 8 * 128 + 1, dtype=BF, device=DEV)[1:].view(8, 16, 8, 128)
@@ -296,6 +297,35 @@ def test_two_recorded_decodes_side_by_side():
     torch.cuda.synchronize()
     assert not outs[0].any()
     for graph in graphs:
+        graph.reset()
+
+
+def test_recorded_behind_a_fork():
+    """Behind work of two streams, a copy and a fill, with a workspace of the call's own and a given one."""
+    b = Batch([4000, 3, 700], 32, 8, 128, BF)
+    want = b.call()
+    ws = torch.zeros(N.load().fq_dense_paged_decode_workspace_bytes(3, 32, 8, 128), dtype=torch.uint8, device=DEV)
+    q, side, main = b.q.clone(), torch.cuda.Stream(), torch.cuda.Stream()
+    main.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(main):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=main):
+            b.q.zero_()
+            side.wait_stream(main)
+            with torch.cuda.stream(side):
+                b.q.copy_(q)
+                lens = b.sl + 0
+                one = fq.split_k_paged_decode_dense(b.q, b.k, b.v, b.table, lens, workspace=ws)
+            two = fq.split_k_paged_decode_dense(q, b.k, b.v, b.table, b.sl)
+            main.wait_stream(side)
+            three = fq.split_k_paged_decode_dense(b.q, b.k, b.v, b.table, lens, workspace=ws)
+            four = three * 1
+        for _ in range(10):
+            for x in (one, two, three, four):
+                x.zero_()
+            graph.replay()
+            main.synchronize()
+            assert all(torch.equal(x, want) for x in (one, two, three, four))
         graph.reset()
 
 
@@ -618,6 +648,7 @@ def test_append_refusals():
     refused(value_cache=vc[:2])
     refused(key_cache=kc.half())
     refused(key_cache=kc[:, :1].expand(3, 16, 4, 64))
+    refused(value_cache=vc.as_strided((3, 16, 4, 64), (4096, 64, 64, 1)))
     refused(slot_mapping=i[:3])
     refused(slot_mapping=i.float())
     refused(positions=None)
