@@ -556,6 +556,16 @@ PyObject* cache_update(PyObject*, Args a, Py_ssize_t n) {
 // ------------------------------------------------------------------------------------
 // around 16-bit pages
 // ------------------------------------------------------------------------------------
+// A contiguous tensor in the bytes of `base` from `offset` on: the results of a call that are used together come from
+// one allocation (1.2 us of host time each).
+Tensor carve(const Tensor& base, int64_t offset, at::IntArrayRef sizes, at::ScalarType st) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()),
+                                                      c10::DispatchKeySet(c10::DispatchKey::CUDA),
+                                                      c10::scalarTypeToTypeMeta(st));
+  t.unsafeGetTensorImpl()->set_storage_offset(offset / int64_t(c10::elementSize(st)));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  return t;
+}
 // (tokens, heads, head_dim) with adjacent values of a head
 const Tensor* rows(PyObject* o, int dev) {
   const Tensor* t = on_device(o, dev);
@@ -632,7 +642,14 @@ PyObject* rotary_embed(PyObject*, Args a, Py_ssize_t n) {
     ok = PyTuple_GET_ITEM(a[7], 1);
   }
   Tensor q_out, k_out;
-  if (!out_rows(oq, *q, dev, q_out) || (k ? !out_rows(ok, *k, dev, k_out) : ok != Py_None)) return none();
+  if (k && oq == Py_None && ok == Py_None) {
+    const int64_t size = int64_t(q->element_size()), first = (q->numel() * size + 255) / 256 * 256;
+    const Tensor both = at::empty({first + k->numel() * size}, q->options().dtype(at::kByte));
+    q_out = carve(both, 0, q->sizes(), q->scalar_type());
+    k_out = carve(both, first, k->sizes(), k->scalar_type());
+  } else if (!out_rows(oq, *q, dev, q_out) || (k ? !out_rows(ok, *k, dev, k_out) : ok != Py_None)) {
+    return none();
+  }
   const int64_t strides[8] = {q->stride(0), q->stride(1), k ? k->stride(0) : 0, k ? k->stride(1) : 0,
                               q_out.stride(0), q_out.stride(1), k ? k_out.stride(0) : 0, k ? k_out.stride(1) : 0};
   const int rc = native(nullptr, [&] {
@@ -762,7 +779,6 @@ PyObject* plan_paged_step(PyObject*, Args a, Py_ssize_t n) {
   if (!context || !query || context->dim() != 1 || query->dim() != 1 || context->size(0) != p.requests ||
       query->size(0) != p.requests)
     return none();
-  // one allocation for all results (an allocation each: 5 us more)
   const auto part = [](int64_t n) { return (n + 15) / 16 * 16; };
   const int64_t r = p.requests, sizes[6] = {4 * r, 4 * (r + 1), 8 * room, 8 * room, r, 4};
   int64_t bytes = 0;
@@ -771,13 +787,9 @@ PyObject* plan_paged_step(PyObject*, Args a, Py_ssize_t n) {
   int64_t offset = 0;
   int made = 0;
   const auto piece = [&](int64_t n, at::ScalarType st) {
-    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()),
-                                                        c10::DispatchKeySet(c10::DispatchKey::CUDA),
-                                                        c10::scalarTypeToTypeMeta(st));
-    t.unsafeGetTensorImpl()->set_storage_offset(offset / int64_t(c10::elementSize(st)));
-    t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
-    offset += part(sizes[made++]);
-    return t;
+    offset += made ? part(sizes[made - 1]) : 0;
+    ++made;
+    return carve(all, offset, {n}, st);
   };
   Tensor out[6];
   out[0] = piece(r, at::kInt);
