@@ -48,11 +48,14 @@ struct DenseArgs {
   int64_t k_block, k_token, k_head, v_block, v_token, v_head;
   int64_t table_stride, num_blocks;
   int seqs, hq, hkv, table_width, block_size, window;
-  int chunks, rows;                      // units of a KV head, query heads of a unit
-  int side, piece_floats;                // units side by side; stride of the pieces
+  int chunks, rows, group;               // units of a KV head, query heads of a unit and of a KV head
+  int side_bits, unit_groups;            // units side by side (a power of two), such groups of a sequence
+  int piece_floats;                      // stride of the pieces
   float scale_log2;
   int fixed;                             // runs dealt out beforehand
-  int join_rows, join_wide;              // heads and dimensions of a CTA of the join
+  int join_rows, join_wide, join_wides;  // heads and dimensions of a CTA of the join, such parts of a head
+  int join_columns, join_groups;         // its columns of four dimensions, threads to each of them
+  int join_split;                        // CTAs of its cluster
   uint32_t *status, *tickets;
   int* bounds;
   float* pieces;                         // [slot][side]: [rows][D], [rows][2] (maximum, sum)
@@ -139,8 +142,8 @@ struct DenseUnit {
   int head0, count;  // query heads
 };
 __device__ __forceinline__ DenseUnit dense_unit(const DenseArgs& p, int unit) {
-  const int group = p.hq / p.hkv, kv = unit / p.chunks, chunk = unit - kv * p.chunks;
-  return {kv * group + chunk * p.rows, min(p.rows, group - chunk * p.rows)};
+  const int kv = p.chunks == 1 ? unit : unit / p.chunks, chunk = unit - kv * p.chunks;
+  return {kv * p.group + chunk * p.rows, min(p.rows, p.group - chunk * p.rows)};
 }
 __device__ __forceinline__ float dense_lse(float m, float l, float lift) {
   return l == 0.f ? -INFINITY : (m + log2f(l) - lift) * 0.69314718f;
@@ -160,7 +163,7 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int g = lane >> 2, t = lane & 3;
   const int64_t room = int64_t(p.table_width) * p.block_size;
-  const int unit_groups = p.hkv * p.chunks / p.side;
+  const int unit_groups = p.unit_groups;
   // (the wait first: the second kernel, which this lets start, reads what the kernels before this one have written)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -200,10 +203,10 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
 
   // ---- the warp's tiles, described sixteen at a time ---------------------------------------------------
   const int tiles_per_block = p.block_size / kDenseTile;
-  const uint32_t taken = uint32_t(cut.taken()) * p.side;
+  const uint32_t taken = uint32_t(cut.taken()) << p.side_bits;
   int4* const mine = described + warp * 32;
   const int here = blockIdx.x * S::kWarps + warp;
-  int run = here / p.side, member = here - run * p.side;
+  int run = here >> p.side_bits, member = here - (run << p.side_bits);
   int at = cut.begin(run), end = cut.end(run);
   uint32_t ticket = 0;  // (lane 0) the next run, where it has been asked for
   bool asked = false;
@@ -226,8 +229,8 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
         finished = true;
         return;
       }
-      run = cut.fixed + x / p.side;
-      member = x % p.side;
+      run = cut.fixed + int(x >> p.side_bits);
+      member = x & ((1 << p.side_bits) - 1);
       at = cut.begin(run);
       end = cut.end(run);
     }
@@ -248,11 +251,11 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
       next.x = __ldg(p.table + lo * p.table_stride + page);
       next.y = (tile - page * tiles_per_block) * kDenseTile | max(span.begin - first, 0) << 22 |
                min(span.len - first, kDenseTile) << 26;
-      next.z = lo | (group * p.side + member) << 12;
+      next.z = lo | ((group << p.side_bits) + member) << 12;
       if (i == cut.kind_of(tail, a) || i == cut.begin(run)) next.z |= 1 << 30;
       if (i + 1 == cut.kind_of(tail, b) || i + 1 == end) next.z |= 1 << 31;
       const int nth = lo * unit_groups + group;
-      next.w = dense_whole(cut, run, a, b) ? -1 : dense_slot(cut, run, nth, p.seqs * unit_groups) * p.side + member;
+      next.w = dense_whole(cut, run, a, b) ? -1 : (dense_slot(cut, run, nth, p.seqs * unit_groups) << p.side_bits) + member;
     }
     at += waiting;
   };
@@ -281,7 +284,7 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
     if (issued < made) {
       const int4 d = mine[issued & 31];
       ++issued;
-      const int head = ((d.z >> 12) & 0x3fff) / p.chunks;
+      const int unit = (d.z >> 12) & 0x3fff, head = p.chunks == 1 ? unit : unit / p.chunks;
       const int row = d.y & (kDenseMaxBlock - 1);
       const int64_t id = d.x < 0 ? 0 : d.x;
       const T* k = static_cast<const T*>(p.k) + id * p.k_block + row * p.k_token + head * p.k_head;
@@ -493,24 +496,28 @@ __global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const Dense
   __shared__ float4 sums[kJoinThreads];
   const cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int units = p.hkv * p.chunks, unit_groups = units / p.side;
-  const int seq = blockIdx.x / units, unit = blockIdx.x - seq * units;
-  const int group = unit / p.side, member = unit - group * p.side;
+  const int unit_groups = p.unit_groups, unit = blockIdx.x, seq = blockIdx.z / p.join_split;
+  const unsigned part = blockIdx.z - seq * p.join_split, parts = p.join_split;  // of the pieces
+  const int group = unit >> p.side_bits, member = unit - (group << p.side_bits);
   const DenseUnit u = dense_unit(p, unit);
-  const int wides = D / p.join_wide, row0 = blockIdx.y / wides * p.join_rows;
+  const int row0 = blockIdx.y / p.join_wides * p.join_rows, wide = blockIdx.y % p.join_wides;
   const int rows = min(p.join_rows, u.count - row0);
-  const int columns = p.join_rows * p.join_wide / 4, groups = kJoinThreads / columns;  // float4
+  const int columns = p.join_columns, groups = p.join_groups;
   const int mine = tid / columns, column = tid - mine * columns;
   const int row = column * 4 / p.join_wide;
-  const int dim = (blockIdx.y % wides) * p.join_wide + column * 4 - row * p.join_wide;
+  const int dim = wide * p.join_wide + column * 4 - row * p.join_wide;
   const bool real = row < rows && mine < groups;
   const int64_t out_row = int64_t(seq) * p.hq + u.head0 + row0;
   int s0, tiles, total;
-  if (p.seqs <= kJoinThreads) {
+  if (p.seqs <= 4 * kJoinThreads) {
     const int64_t room = int64_t(p.table_width) * p.block_size;
-    const int own = tid < p.seqs ? dense_span(p.lens[tid], room, p.window).tiles : 0;
     tiles = dense_span(p.lens[seq], room, p.window).tiles;
-    int all = own, before = tid < seq ? own : 0;
+    int all = 0, before = 0;
+    for (int s = tid; s < p.seqs; s += kJoinThreads) {
+      const int own = dense_span(p.lens[s], room, p.window).tiles;
+      all += own;
+      if (s < seq) before += own;
+    }
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) {
       all += __shfl_xor_sync(0xffffffffu, all, s);
@@ -539,21 +546,21 @@ __global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const Dense
     x.y = Dense16<T>::pack(o.z, o.w);
     *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (out_row + row) * D + dim) = x;
   };
-  const bool with_lse = p.lse && blockIdx.y % wides == 0 && blockIdx.z == 0;
+  const bool with_lse = p.lse && wide == 0 && part == 0;
   const DenseCut cut = dense_cut(total, p.fixed);
   const int a = s0 + group * tiles;
   const DensePieces all = dense_pieces(cut, a, a + tiles);
-  const int pieces = all.count(), first = pieces * blockIdx.z / gridDim.z, n = pieces * (blockIdx.z + 1) / gridDim.z;
+  const int pieces = all.count(), first = pieces * part / parts, n = pieces * (part + 1) / parts;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (tiles == 0 && blockIdx.z == 0) {
+  if (tiles == 0 && part == 0) {
     if (real && mine == 0) write(make_float4(0.f, 0.f, 0.f, 0.f));
     if (with_lse && tid < rows) p.lse[out_row + tid] = -INFINITY;
   }
   if (tiles == 0 || pieces == 1 || rows <= 0) return;
   const int nth = seq * unit_groups + group, groups_all = p.seqs * unit_groups;
   auto piece = [&](int i) {
-    return p.pieces + (int64_t(dense_slot(cut, all.run(i), nth, groups_all)) * p.side + member) * p.piece_floats;
+    return p.pieces + ((int64_t(dense_slot(cut, all.run(i), nth, groups_all)) << p.side_bits) + member) * p.piece_floats;
   };
   const int64_t offset = (row0 + row) * D + dim;
   float m = -INFINITY, l = 0.f;  // of row `warp`
@@ -625,14 +632,14 @@ __global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const Dense
     for (int i = 1; i < groups; ++i) add(1.f, sums[i * columns + column]);
     sums[tid] = o;
   }
-  if (gridDim.z > 1) cluster_barrier();
-  if (blockIdx.z == 0) {
+  if (parts > 1) cluster_barrier();
+  if (part == 0) {
     float top = -INFINITY, sum = 0.f;  // of all CTAs, of the thread's row
     if (real && mine == 0) {
-      for (unsigned z = 0; z < gridDim.z; ++z) top = fmaxf(top, cluster.map_shared_rank(&totals[row][0], z)[0]);
+      for (unsigned z = 0; z < parts; ++z) top = fmaxf(top, cluster.map_shared_rank(&totals[row][0], z)[0]);
       const float ref = top == -INFINITY ? 0.f : top;
       o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (unsigned z = 0; z < gridDim.z; ++z) {
+      for (unsigned z = 0; z < parts; ++z) {
         const float* of = cluster.map_shared_rank(&totals[row][0], z);
         const float w = fast_exp2(of[0] - ref);
         sum = fmaf(w, of[1], sum);
@@ -643,25 +650,25 @@ __global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const Dense
       if (with_lse && column * 4 == row * p.join_wide) p.lse[out_row + row] = dense_lse(top, sum, Dense16<T>::kLift);
     }
   }
-  if (gridDim.z > 1) cluster_barrier();  // what the first CTA reads stays
+  if (parts > 1) cluster_barrier();  // what the first CTA reads stays
 }
 
 // ------------------------------------------------------------------------------------
 // Host side
 // ------------------------------------------------------------------------------------
 struct DenseGeometry {
-  int chunks, rows, side, piece_floats;
+  int chunks, rows, group, side_bits, piece_floats;
   bool r16;
 };
 // Up to 8 query heads to a unit (16 where a KV head has more: its keys are then read half as often).
 static DenseGeometry dense_geometry(int hq, int hkv, int d) {
   DenseGeometry x;
-  const int group = hq / hkv;
-  x.r16 = group > 8;
-  x.chunks = (group + 15) / 16;
-  x.rows = (group + x.chunks - 1) / x.chunks;
-  x.side = dense_warps(d);  // adjacent units to the warps of a CTA, as many as divide a sequence's units
-  while (hkv * x.chunks % x.side != 0) x.side /= 2;
+  x.group = hq / hkv;
+  x.r16 = x.group > 8;
+  x.chunks = (x.group + 15) / 16;
+  x.rows = (x.group + x.chunks - 1) / x.chunks;
+  x.side_bits = 0;  // adjacent units to the warps of a CTA, as many as divide a sequence's units
+  while (2 << x.side_bits <= dense_warps(d) && hkv * x.chunks % (2 << x.side_bits) == 0) ++x.side_bits;
   x.piece_floats = (x.rows * (d + 2) + 3) & ~3;
   return x;
 }
@@ -691,7 +698,7 @@ static int dense_sms(int& sms) {
 // Programmatic dependent launch: the kernel's CTAs may start while the one before it on the stream ends, and wait for it
 // themselves.
 static int launch_dependent(void (*kernel)(DenseArgs), const DenseArgs& p, dim3 grid, int threads, size_t smem,
-                            cudaStream_t stream) {
+                            int cluster, cudaStream_t stream) {
   cudaLaunchConfig_t config = {};
   config.gridDim = grid;
   config.blockDim = dim3(threads);
@@ -702,9 +709,9 @@ static int launch_dependent(void (*kernel)(DenseArgs), const DenseArgs& p, dim3 
   attributes[0].val.programmaticStreamSerializationAllowed = 1;
   attributes[1].id = cudaLaunchAttributeClusterDimension;  // the CTAs along z
   attributes[1].val.clusterDim.x = attributes[1].val.clusterDim.y = 1;
-  attributes[1].val.clusterDim.z = grid.z;
+  attributes[1].val.clusterDim.z = cluster;
   config.attrs = attributes;
-  config.numAttrs = grid.z > 1 ? 2 : 1;
+  config.numAttrs = cluster > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&config, kernel, p);
   if (e != cudaSuccess) return fail(FQ_ERR_CUDA, "dense decode: %s", cudaGetErrorString(e));
   return check_launch("dense decode");
@@ -724,12 +731,15 @@ static int launch_join(DenseArgs p, cudaStream_t stream) {
   while (p.join_rows < p.rows && 2 * p.join_rows <= kJoinRows && 2 * p.join_rows * p.join_wide / 4 <= kJoinThreads &&
          ctas() > most)
     p.join_rows *= 2;
-  const unsigned parts = (p.rows + p.join_rows - 1) / p.join_rows * (D / p.join_wide);
+  p.join_wides = D / p.join_wide;
+  p.join_columns = p.join_rows * p.join_wide / 4;
+  p.join_groups = kJoinThreads / p.join_columns;
   const int64_t tiles = int64_t(p.table_width) * (p.block_size / kDenseTile);
-  const int64_t pieces = std::min(tiles, int64_t(p.fixed) * (1 + kDenseTaken) * p.side / units);  // of a unit, about
-  unsigned split = 1;
-  while (split < 8 && pieces > 64 * split && 2 * split * ctas() <= most) split *= 2;
-  return launch_dependent(dense_join_kernel<T, D>, p, dim3(unsigned(units), parts, split), kJoinThreads, 0, stream);
+  const int64_t pieces = std::min(tiles, (int64_t(p.fixed) * (1 + kDenseTaken) << p.side_bits) / units);  // of a unit, about
+  p.join_split = 1;
+  while (p.join_split < 8 && pieces > 64 * p.join_split && 2 * p.join_split * ctas() <= most) p.join_split *= 2;
+  const dim3 grid(p.hkv * p.chunks, (p.rows + p.join_rows - 1) / p.join_rows * p.join_wides, p.seqs * p.join_split);
+  return launch_dependent(dense_join_kernel<T, D>, p, grid, kJoinThreads, 0, p.join_split, stream);
 }
 
 template <typename T, int D, bool R16>
@@ -748,7 +758,7 @@ static int launch_dense(const DenseArgs& p, int ctas, cudaStream_t stream) {
       return fail(FQ_ERR_CUDA, "dense decode: %s", cudaGetErrorString(e));
     }
   }
-  if (const int rc = launch_dependent(kernel, p, dim3(ctas), S::kWarps * 32, smem, stream)) return rc;
+  if (const int rc = launch_dependent(kernel, p, dim3(ctas), S::kWarps * 32, smem, 1, stream)) return rc;
   return launch_join<T, D>(p, stream);
 }
 template <typename T, int D>
@@ -778,8 +788,8 @@ extern "C" size_t fq_dense_paged_decode_workspace_bytes(int num_seqs, int num_q_
                                                         int head_dim) {
   if (!dense_shape_ok(num_seqs, num_q_heads, num_kv_heads, head_dim)) return 0;
   const DenseGeometry x = dense_geometry(num_q_heads, num_kv_heads, head_dim);
-  const int teams = dense_warps(head_dim) / x.side, groups = num_kv_heads * x.chunks / x.side;
-  return kDensePieces + dense_slots(kDenseMaxCtas * teams, num_seqs * groups) * x.side * size_t(x.piece_floats) * sizeof(float);
+  const int teams = dense_warps(head_dim) >> x.side_bits, groups = num_kv_heads * x.chunks >> x.side_bits;
+  return kDensePieces + (dense_slots(kDenseMaxCtas * teams, num_seqs * groups) << x.side_bits) * size_t(x.piece_floats) * sizeof(float);
 }
 
 extern "C" int fq_dense_paged_decode(
@@ -810,7 +820,7 @@ extern "C" int fq_dense_paged_decode(
   FQ_REQUIRE(aligned(q, 4) && (q_seq_stride | q_head_stride) % 2 == 0 && aligned(out, 8), FQ_ERR_ALIGNMENT,
              "dense decode: rows of q must start at multiples of 4 bytes, out at one of 8");
   const DenseGeometry x = dense_geometry(num_q_heads, num_kv_heads, head_dim);
-  const int64_t unit_groups = int64_t(num_kv_heads) * x.chunks / x.side;
+  const int64_t unit_groups = int64_t(num_kv_heads) * x.chunks >> x.side_bits;
   const int64_t most = num_seqs * unit_groups * block_table_width * (block_size / kDenseTile);
   FQ_REQUIRE(most < (int64_t(1) << 30), FQ_ERR_UNSUPPORTED, "dense decode: block table of 2^30 tiles or more");
   FQ_REQUIRE(workspace && aligned(workspace, 16) &&
@@ -825,7 +835,8 @@ extern "C" int fq_dense_paged_decode(
   p.table_stride = block_table_stride; p.num_blocks = num_blocks;
   p.seqs = num_seqs; p.hq = num_q_heads; p.hkv = num_kv_heads;
   p.table_width = block_table_width; p.block_size = block_size; p.window = window;
-  p.chunks = x.chunks; p.rows = x.rows; p.side = x.side; p.piece_floats = x.piece_floats;
+  p.chunks = x.chunks; p.rows = x.rows; p.group = x.group; p.side_bits = x.side_bits;
+  p.unit_groups = int(unit_groups); p.piece_floats = x.piece_floats;
   p.scale_log2 = sm_scale * 1.44269504f;
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   p.status = reinterpret_cast<uint32_t*>(ws);
@@ -835,7 +846,7 @@ extern "C" int fq_dense_paged_decode(
   // one CTA per SM (the rings fill its shared memory), no more than there can be runs
   int sms = 0;
   if (const int rc = dense_sms(sms)) return rc;
-  const int teams = dense_warps(head_dim) / x.side;
+  const int teams = dense_warps(head_dim) >> x.side_bits;
   const int64_t runs = (most + kDenseShortest - 1) / kDenseShortest;
   const int ctas = int(std::max<int64_t>(1, std::min<int64_t>(sms, (runs + teams - 1) / teams)));
   p.fixed = ctas * teams;
