@@ -255,23 +255,35 @@ static int launch_rotary(const RotaryArgs& p, bool half_layout, cudaStream_t str
   const int jobs = RotaryJobs(all, p.q.heads, rows).count + RotaryJobs(all, p.k.heads, rows).count +
                    RotaryJobs(all_v, p.v.heads, rows).count;
   const int groups = (jobs + kRotWarps - 1) / kRotWarps, warps = (jobs + groups - 1) / groups;
-  // A few tokens are spread over more CTAs.  (590 tokens of 40 heads: 4.3, 4.1, 5.3 us with 1, 2, 4 at a time, 148: 3.1,
-  // 3.8, 5.2, 8192: 35.1, 32.2, 32.7, 16384: 66.2, 60.6, 58.4.)
-  const int batch = p.tokens <= 592 ? 1 : (p.tokens <= 1184 ? 2 : kRotTokens);
-  const size_t smem = 2 * size_t(batch) * (p.rotary_dim / 2) * sizeof(float2);
   const auto kernel = wide ? (half_layout ? rotary_kernel<T, N, true> : rotary_kernel<T, N, false>)
                            : (half_layout ? rotary_kernel<T, 1, true> : rotary_kernel<T, 1, false>);
-  // no more CTAs than are resident together
+  const auto smem = [&](int batch) { return 2 * size_t(batch) * (p.rotary_dim / 2) * sizeof(float2); };
+  // A few tokens are spread over more CTAs.  (590 tokens of 40 heads: 4.3, 4.1, 5.3 us with 1, 2, 4 at a time, 148: 3.1,
+  // 3.8, 5.2, 8192: 35.1, 32.2, 32.7, 16384: 66.2, 60.6, 58.4.)
+  int batch = p.tokens <= 592 ? 1 : 2;
   int64_t ctas = (p.tokens + batch - 1) / batch;
-  if (ctas > 64) {
+  if (ctas > 64) {  // no more CTAs than are resident together
     int device = 0, sms = 0, fit = 0;
     cudaError_t e = cudaGetDevice(&device);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, warps * 32, smem);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, warps * 32, smem(kRotTokens));
     if (e != cudaSuccess) return fail(FQ_ERR_CUDA, "rotary: %s", cudaGetErrorString(e));
-    ctas = std::min<int64_t>(ctas, std::max(1, sms * fit / groups));
+    const int64_t most = std::max(1, sms * fit / groups);
+    if (p.tokens > 1184) {
+      // what leaves the last round of the CTAs fullest, a token less at a time counted as 2 % more work (8192 tokens:
+      // 31.7 us with 4, 30.6 with 3; of heads of 64 19.6 and 18.4)
+      int64_t least = INT64_MAX;
+      for (int n = kRotTokens; n > 1; --n) {
+        const int64_t rounds = ((p.tokens + n - 1) / n + most - 1) / most, cost = rounds * n * (50 + kRotTokens - n);
+        if (cost < least) {
+          least = cost;
+          batch = n;
+        }
+      }
+    }
+    ctas = std::min((p.tokens + batch - 1) / batch, most);
   }
-  kernel<<<dim3(unsigned(ctas), groups), warps * 32, smem, stream>>>(p, batch);
+  kernel<<<dim3(unsigned(ctas), groups), warps * 32, smem(batch), stream>>>(p, batch);
   return check_launch("rotary");
 }
 
