@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
   cp_async_wait<0>();
 }
 
-// A cluster for `join_rows` query heads of a unit and `join_wide` of their dimensions, each of its CTAs for a part of the
+// A cluster for `join_rows` query heads of a unit, or of a few units one after the other, and `join_wide` of their dimensions, each of its CTAs for a part of the
 // pieces: their weights first, a warp to a head and a lane to a piece, then the sums, a group of threads to a piece, and
 // the first CTA adds up what the others have in their shared memory.  A unit that one run had is left alone; heads without
 // tokens get zeros.  What does not depend on the pieces is done before the wait for the first kernel, and the first pieces
@@ -496,18 +496,13 @@ __global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const Dense
   __shared__ float4 sums[kJoinThreads];
   const cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int unit_groups = p.unit_groups, unit = blockIdx.x, seq = blockIdx.z / p.join_split;
+  const int unit_groups = p.unit_groups, units = unit_groups << p.side_bits, seq = blockIdx.z / p.join_split;
   const unsigned part = blockIdx.z - seq * p.join_split, parts = p.join_split;  // of the pieces
-  const int group = unit >> p.side_bits, member = unit - (group << p.side_bits);
-  const DenseUnit u = dense_unit(p, unit);
   const int row0 = blockIdx.y / p.join_wides * p.join_rows, wide = blockIdx.y % p.join_wides;
-  const int rows = min(p.join_rows, u.count - row0);
   const int columns = p.join_columns, groups = p.join_groups;
   const int mine = tid / columns, column = tid - mine * columns;
   const int row = column * 4 / p.join_wide;
   const int dim = wide * p.join_wide + column * 4 - row * p.join_wide;
-  const bool real = row < rows && mine < groups;
-  const int64_t out_row = int64_t(seq) * p.hq + u.head0 + row0;
   int s0, tiles, total;
   if (p.seqs <= 4 * kJoinThreads) {
     const int64_t room = int64_t(p.table_width) * p.block_size;
@@ -540,117 +535,125 @@ __global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const Dense
     tiles = (p.bounds[seq + 1] - s0) / unit_groups;
     total = p.bounds[p.seqs];
   }
-  auto write = [&](float4 o) {
-    uint2 x;
-    x.x = Dense16<T>::pack(o.x, o.y);
-    x.y = Dense16<T>::pack(o.z, o.w);
-    *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (out_row + row) * D + dim) = x;
-  };
   const bool with_lse = p.lse && wide == 0 && part == 0;
   const DenseCut cut = dense_cut(total, p.fixed);
-  const int a = s0 + group * tiles;
-  const DensePieces all = dense_pieces(cut, a, a + tiles);
-  const int pieces = all.count(), first = pieces * part / parts, n = pieces * (part + 1) / parts;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (tiles == 0 && part == 0) {
-    if (real && mine == 0) write(make_float4(0.f, 0.f, 0.f, 0.f));
-    if (with_lse && tid < rows) p.lse[out_row + tid] = -INFINITY;
-  }
-  if (tiles == 0 || pieces == 1 || rows <= 0) return;
-  const int nth = seq * unit_groups + group, groups_all = p.seqs * unit_groups;
-  auto piece = [&](int i) {
-    return p.pieces + ((int64_t(dense_slot(cut, all.run(i), nth, groups_all)) << p.side_bits) + member) * p.piece_floats;
-  };
-  const int64_t offset = (row0 + row) * D + dim;
-  float m = -INFINITY, l = 0.f;  // of row `warp`
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](float w, const float4& v) {
-    o.x = fmaf(w, v.x, o.x);
-    o.y = fmaf(w, v.y, o.y);
-    o.z = fmaf(w, v.z, o.z);
-    o.w = fmaf(w, v.w, o.w);
-  };
-  if (tid < kJoinRows) {
-    totals[tid][0] = -INFINITY;
-    totals[tid][1] = 0.f;
-  }
-  for (int i0 = first; i0 < n; i0 += kJoinPieces) {
-    const int some = min(kJoinPieces, n - i0);
-    float4 ahead[kAhead];
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int i = mine + k * groups;
-      if (real && i < some) ahead[k] = *reinterpret_cast<const float4*>(piece(i0 + i) + offset);
+  for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const int group = unit >> p.side_bits, member = unit - (group << p.side_bits);
+    const DenseUnit u = dense_unit(p, unit);
+    const int rows = min(p.join_rows, u.count - row0);
+    const bool real = row < rows && mine < groups;
+    const int64_t out_row = int64_t(seq) * p.hq + u.head0 + row0;
+    auto write = [&](float4 o) {
+      uint2 x;
+      x.x = Dense16<T>::pack(o.x, o.y);
+      x.y = Dense16<T>::pack(o.z, o.w);
+      *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (out_row + row) * D + dim) = x;
+    };
+    const int a = s0 + group * tiles;
+    const DensePieces all = dense_pieces(cut, a, a + tiles);
+    const int pieces = all.count(), first = pieces * part / parts, n = pieces * (part + 1) / parts;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // (passed at once from the second unit on)
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (tiles == 0 && part == 0) {
+      if (real && mine == 0) write(make_float4(0.f, 0.f, 0.f, 0.f));
+      if (with_lse && tid < rows) p.lse[out_row + tid] = -INFINITY;
     }
-    __syncthreads();  // the weights before have been used
-    if (warp < rows) {
-      float2 x[kJoinPieces / 32];
-      float now = m;
-#pragma unroll
-      for (int k = 0; k < kJoinPieces / 32; ++k) {
-        const int i = lane + 32 * k;
-        x[k] = make_float2(-INFINITY, 0.f);
-        if (i < some) x[k] = *reinterpret_cast<const float2*>(piece(i0 + i) + p.rows * D + 2 * (row0 + warp));
-      }
-#pragma unroll
-      for (int k = 0; k < kJoinPieces / 32; ++k) now = fmaxf(now, x[k].x);
-#pragma unroll
-      for (int s = 16; s > 0; s >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, s));
-      const float ref = now == -INFINITY ? 0.f : now, f = fast_exp2(m - ref);
-      float s = 0.f;
-#pragma unroll
-      for (int k = 0; k < kJoinPieces / 32; ++k) {
-        const float w = fast_exp2(x[k].x - ref);
-        s = fmaf(w, x[k].y, s);
-        weights[warp][lane + 32 * k] = w;
-      }
-      l = fmaf(l, f, warp_sum(s));
-      m = now;
-      if (lane == 0) {
-        totals[warp][0] = m;
-        totals[warp][1] = l;
-        totals[warp][2] = f;
-      }
+    if (tiles == 0 || pieces == 1 || rows <= 0) continue;
+    __syncthreads();  // what the unit before had in shared memory has been read
+    const int nth = seq * unit_groups + group, groups_all = p.seqs * unit_groups;
+    auto piece = [&](int i) {
+      return p.pieces + ((int64_t(dense_slot(cut, all.run(i), nth, groups_all)) << p.side_bits) + member) * p.piece_floats;
+    };
+    const int64_t offset = (row0 + row) * D + dim;
+    float m = -INFINITY, l = 0.f;  // of row `warp`
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float w, const float4& v) {
+      o.x = fmaf(w, v.x, o.x);
+      o.y = fmaf(w, v.y, o.y);
+      o.z = fmaf(w, v.z, o.z);
+      o.w = fmaf(w, v.w, o.w);
+    };
+    if (tid < kJoinRows) {
+      totals[tid][0] = -INFINITY;
+      totals[tid][1] = 0.f;
     }
-    __syncthreads();
-    if (!real) continue;
-    const float f = totals[row][2];
-    o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+    for (int i0 = first; i0 < n; i0 += kJoinPieces) {
+      const int some = min(kJoinPieces, n - i0);
+      float4 ahead[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int i = mine + k * groups;
-      if (i < some) add(weights[row][i], ahead[k]);
-    }
+      for (int k = 0; k < kAhead; ++k) {
+        const int i = mine + k * groups;
+        if (real && i < some) ahead[k] = *reinterpret_cast<const float4*>(piece(i0 + i) + offset);
+      }
+      __syncthreads();  // the weights before have been used
+      if (warp < rows) {
+        float2 x[kJoinPieces / 32];
+        float now = m;
+#pragma unroll
+        for (int k = 0; k < kJoinPieces / 32; ++k) {
+          const int i = lane + 32 * k;
+          x[k] = make_float2(-INFINITY, 0.f);
+          if (i < some) x[k] = *reinterpret_cast<const float2*>(piece(i0 + i) + p.rows * D + 2 * (row0 + warp));
+        }
+#pragma unroll
+        for (int k = 0; k < kJoinPieces / 32; ++k) now = fmaxf(now, x[k].x);
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, s));
+        const float ref = now == -INFINITY ? 0.f : now, f = fast_exp2(m - ref);
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < kJoinPieces / 32; ++k) {
+          const float w = fast_exp2(x[k].x - ref);
+          s = fmaf(w, x[k].y, s);
+          weights[warp][lane + 32 * k] = w;
+        }
+        l = fmaf(l, f, warp_sum(s));
+        m = now;
+        if (lane == 0) {
+          totals[warp][0] = m;
+          totals[warp][1] = l;
+          totals[warp][2] = f;
+        }
+      }
+      __syncthreads();
+      if (!real) continue;
+      const float f = totals[row][2];
+      o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int i = mine + k * groups;
+        if (i < some) add(weights[row][i], ahead[k]);
+      }
 #pragma unroll 6
-    for (int i = mine + kAhead * groups; i < some; i += groups)
-      add(weights[row][i], *reinterpret_cast<const float4*>(piece(i0 + i) + offset));
-  }
-  sums[tid] = o;
-  __syncthreads();
-  if (real && mine == 0) {
-    for (int i = 1; i < groups; ++i) add(1.f, sums[i * columns + column]);
-    sums[tid] = o;
-  }
-  if (parts > 1) cluster_barrier();
-  if (part == 0) {
-    float top = -INFINITY, sum = 0.f;  // of all CTAs, of the thread's row
-    if (real && mine == 0) {
-      for (unsigned z = 0; z < parts; ++z) top = fmaxf(top, cluster.map_shared_rank(&totals[row][0], z)[0]);
-      const float ref = top == -INFINITY ? 0.f : top;
-      o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (unsigned z = 0; z < parts; ++z) {
-        const float* of = cluster.map_shared_rank(&totals[row][0], z);
-        const float w = fast_exp2(of[0] - ref);
-        sum = fmaf(w, of[1], sum);
-        add(w, *cluster.map_shared_rank(&sums[tid], z));
-      }
-      const float f = sum == 0.f ? 0.f : 1.f / sum;
-      write(make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
-      if (with_lse && column * 4 == row * p.join_wide) p.lse[out_row + row] = dense_lse(top, sum, Dense16<T>::kLift);
+      for (int i = mine + kAhead * groups; i < some; i += groups)
+        add(weights[row][i], *reinterpret_cast<const float4*>(piece(i0 + i) + offset));
     }
+    sums[tid] = o;
+    __syncthreads();
+    if (real && mine == 0) {
+      for (int i = 1; i < groups; ++i) add(1.f, sums[i * columns + column]);
+      sums[tid] = o;
+    }
+    if (parts > 1) cluster_barrier();
+    if (part == 0) {
+      float top = -INFINITY, sum = 0.f;  // of all CTAs, of the thread's row
+      if (real && mine == 0) {
+        for (unsigned z = 0; z < parts; ++z) top = fmaxf(top, cluster.map_shared_rank(&totals[row][0], z)[0]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (unsigned z = 0; z < parts; ++z) {
+          const float* of = cluster.map_shared_rank(&totals[row][0], z);
+          const float w = fast_exp2(of[0] - ref);
+          sum = fmaf(w, of[1], sum);
+          add(w, *cluster.map_shared_rank(&sums[tid], z));
+        }
+        const float f = sum == 0.f ? 0.f : 1.f / sum;
+        write(make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+        if (with_lse && column * 4 == row * p.join_wide) p.lse[out_row + row] = dense_lse(top, sum, Dense16<T>::kLift);
+      }
+    }
+    if (parts > 1) cluster_barrier();  // what the first CTA reads stays
   }
-  if (parts > 1) cluster_barrier();  // what the first CTA reads stays
 }
 
 // ------------------------------------------------------------------------------------
@@ -738,7 +741,8 @@ static int launch_join(DenseArgs p, cudaStream_t stream) {
   const int64_t pieces = std::min(tiles, (int64_t(p.fixed) * (1 + kDenseTaken) << p.side_bits) / units);  // of a unit, about
   p.join_split = 1;
   while (p.join_split < 8 && pieces > 64 * p.join_split && 2 * p.join_split * ctas() <= most) p.join_split *= 2;
-  const dim3 grid(p.hkv * p.chunks, (p.rows + p.join_rows - 1) / p.join_rows * p.join_wides, p.seqs * p.join_split);
+  const int64_t over = (ctas() + most - 1) / most;  // units of a sequence that a CTA takes
+  const dim3 grid(unsigned((p.hkv * p.chunks + over - 1) / over), (p.rows + p.join_rows - 1) / p.join_rows * p.join_wides, p.seqs * p.join_split);
   return launch_dependent(dense_join_kernel<T, D>, p, grid, kJoinThreads, 0, p.join_split, stream);
 }
 
