@@ -199,7 +199,8 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
     if (blockIdx.x == 0 && tid == 0) p.bounds[0] = 0;
     __syncthreads();
   }
-  const DenseCut cut = dense_cut(prefix[p.seqs], p.fixed);
+  const int groups_all = p.seqs * unit_groups;
+  const DenseCut cut = dense_cut(prefix[p.seqs], p.fixed, groups_all);
 
   // ---- the warp's tiles, described sixteen at a time ---------------------------------------------------
   const int tiles_per_block = p.block_size / kDenseTile;
@@ -255,7 +256,7 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
       if (i == cut.kind_of(tail, a) || i == cut.begin(run)) next.z |= 1 << 30;
       if (i + 1 == cut.kind_of(tail, b) || i + 1 == end) next.z |= 1 << 31;
       const int nth = lo * unit_groups + group;
-      next.w = dense_whole(cut, run, a, b) ? -1 : (dense_slot(cut, run, nth, p.seqs * unit_groups) << p.side_bits) + member;
+      next.w = dense_whole(cut, run, a, b) ? -1 : (dense_slot(cut, run, nth, groups_all, a) << p.side_bits) + member;
     }
     at += waiting;
   };
@@ -536,7 +537,8 @@ __global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const Dense
     total = p.bounds[p.seqs];
   }
   const bool with_lse = p.lse && wide == 0 && part == 0;
-  const DenseCut cut = dense_cut(total, p.fixed);
+  const int groups_all = p.seqs * unit_groups;
+  const DenseCut cut = dense_cut(total, p.fixed, groups_all);
   for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
     const int group = unit >> p.side_bits, member = unit - (group << p.side_bits);
     const DenseUnit u = dense_unit(p, unit);
@@ -560,9 +562,9 @@ __global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const Dense
     }
     if (tiles == 0 || pieces == 1 || rows <= 0) continue;
     __syncthreads();  // what the unit before had in shared memory has been read
-    const int nth = seq * unit_groups + group, groups_all = p.seqs * unit_groups;
+    const int nth = seq * unit_groups + group;
     auto piece = [&](int i) {
-      return p.pieces + ((int64_t(dense_slot(cut, all.run(i), nth, groups_all)) << p.side_bits) + member) * p.piece_floats;
+      return p.pieces + ((int64_t(dense_slot(cut, all.run(i), nth, groups_all, a)) << p.side_bits) + member) * p.piece_floats;
     };
     const int64_t offset = (row0 + row) * D + dim;
     float m = -INFINITY, l = 0.f;  // of row `warp`
@@ -792,8 +794,8 @@ extern "C" size_t fq_dense_paged_decode_workspace_bytes(int num_seqs, int num_q_
                                                         int head_dim) {
   if (!dense_shape_ok(num_seqs, num_q_heads, num_kv_heads, head_dim)) return 0;
   const DenseGeometry x = dense_geometry(num_q_heads, num_kv_heads, head_dim);
-  const int teams = dense_warps(head_dim) >> x.side_bits, groups = num_kv_heads * x.chunks >> x.side_bits;
-  return kDensePieces + (dense_slots(kDenseMaxCtas * teams, num_seqs * groups) << x.side_bits) * size_t(x.piece_floats) * sizeof(float);
+  const int teams = dense_warps(head_dim) >> x.side_bits;
+  return kDensePieces + (size_t(dense_slots(kDenseMaxCtas * teams)) << x.side_bits) * x.piece_floats * sizeof(float);
 }
 
 extern "C" int fq_dense_paged_decode(

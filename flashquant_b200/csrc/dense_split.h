@@ -48,6 +48,7 @@ constexpr int kDenseShare = 192;
 constexpr int kDenseMain = 14;    // entries of sixteen that are not in the tail
 constexpr int kDenseTaken = 4;    // runs taken per share, at most
 constexpr int kDenseShortest = 1; // tiles of a run at least
+constexpr int kDenseGroups = 4;   // unit groups to a share from which on there is none (a piece of each is kept room for)
 
 struct DenseCut {
   int total;                  // entries of the list (below 2^30)
@@ -80,12 +81,13 @@ struct DenseCut {
   }
   FQ_HD int taken() const { return (tails + shorter - 1) / shorter; }
 };
-FQ_HD DenseCut dense_cut(int total, int fixed) {
+// `groups`: unit groups of all sequences
+FQ_HD DenseCut dense_cut(int total, int fixed, int groups) {
   DenseCut c;
   const int share = (total + fixed - 1) / fixed;
   c.total = total;
   c.fixed = fixed;
-  c.split = share >= kDenseShare;
+  c.split = share >= kDenseShare && groups <= kDenseGroups * fixed;
   c.mains = c.main_of(total);
   c.tails = total - c.mains;
   c.length = c.split ? (c.mains + fixed - 1) / fixed : share;
@@ -120,12 +122,15 @@ FQ_HD bool dense_whole(const DenseCut& c, int run, int a, int b) {
   return c.kind_of(!tail, a) == c.kind_of(!tail, b) && c.kind_of(tail, a) >= c.begin(run) &&
          c.kind_of(tail, b) <= c.end(run);
 }
-// Where the piece of the `nth` of all `groups` is that a run leaves: along the list of either kind each next piece is
-// of a later run or of a later group, so that the sum of the two counts them.
-FQ_HD int dense_slot(const DenseCut& c, int run, int nth, int groups) {
+// Where the piece of the `nth` group, which takes the entries from `a` on, stands that a run leaves.  Without a tail a run
+// has at most two: of the group that was begun before it and of the one that goes on behind it.  With one, a group that
+// the run has the main entries of is no whole either; but along the list of either kind each next piece is of a later
+// run or of a later group, so that the sum of the two counts them.
+FQ_HD int dense_slot(const DenseCut& c, int run, int nth, int groups, int a) {
+  if (!c.split) return 2 * run + (a < c.begin(run) ? 0 : 1);
   return run + nth + (c.is_tail(run) ? groups : 0);
 }
-// Slots in all, whatever the lengths are: one behind the largest.
-FQ_HD int64_t dense_slots(int fixed, int groups) { return int64_t(fixed) * (1 + kDenseTaken) + 2 * int64_t(groups); }
+// Slots in all, whatever the lengths are.
+FQ_HD int dense_slots(int fixed) { return fixed * (1 + kDenseTaken + 2 * kDenseGroups); }
 
 }  // namespace fq

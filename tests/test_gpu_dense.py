@@ -242,14 +242,14 @@ def test_decode_repeats_bit_for_bit():
 @pytest.mark.parametrize("hq, hkv, d, lens, window", [
     (32, 8, 128, [230001, 3, 131072, 0, 77000, 60123], 0), (8, 1, 128, [1500000, 17, 2300000], 0),
     (16, 16, 64, [300000, 1, 180007, 90000], 0), (20, 2, 256, [70000, 500000, 16, 430000], 0),
-    (32, 8, 128, [400000, 5, 390007], 300000)])
+    (32, 8, 128, [400000, 5, 390007], 300000), (32, 8, 128, [900 - i % 300 for i in range(620)], 0)])
 def test_decode_long_lists(hq, hkv, d, lens, window):
-    """Lists of which warps take a part when they are free (1.9 GB of keys and values): right, and the same bits
-    whoever takes what; the workspace's head is left as it was."""
+    """Lists of which warps take a part when they are free (1.9 GB of keys and values; the last is one of too many
+    sequences for that): right, and the same bits whoever takes what; the workspace's head is left as it was."""
     b = Batch(lens, hq, hkv, d, BF, block=64, window=window)
     ws = torch.zeros(N.load().fq_dense_paged_decode_workspace_bytes(len(lens), hq, hkv, d), dtype=torch.uint8, device=DEV)
     out, lse = b.call(return_lse=True, workspace=ws)
-    b.check(out, lse)
+    b.check(out, lse, only=range(0, len(lens), max(1, len(lens) // 40)))
     for _ in range(15):
         assert torch.equal(b.call(workspace=ws), out)
     assert not ws[:32768].any()
