@@ -19,8 +19,8 @@
 // and one warp had to read all pieces of a long sequence.
 //
 // Measured (us the call, bytes of the keys and values a second): 32 x 4096, 32 / 8 heads of 128: 93, 5.8 TB/s; ragged
-// 8 x 131072, 64 / 8: 430, 6.8; 48 windows of 1000, 16 / 16 heads of 64: 41, 4.8; 64 x 2000, 16 / 8 of 256: 208, 5.0 (four
-// warps with 16 KB a tile: latency); 1 x 900: 9 us, of which the first tile is computed at 5 and the join takes 2.
+// 8 x 131072, 64 / 8: 430, 6.8; 48 windows of 1000, 16 / 16 heads of 64: 41, 4.8; 64 x 2000, 16 / 8 of 256: 168, 6.3; 1 x 900:
+// 9 us, of which the first tile is computed at 5 and the join takes 2.
 #include <algorithm>
 
 #include <cooperative_groups.h>
@@ -65,7 +65,7 @@ struct DenseArgs {
 // 48 x 1000 tokens: 54 us with 8, 39 with 16.
 __host__ __device__ constexpr int dense_warps(int d) { return d == 64 ? 16 : (d > 128 ? 4 : 8); }
 
-template <int D>
+template <int D, bool R16>
 struct DenseShape {
   static constexpr int kWarps = dense_warps(D);
   static constexpr int kRow = 2 * D;         // bytes
@@ -74,7 +74,13 @@ struct DenseShape {
   static constexpr int kStages = D == 96 ? 4 : 3;  // 192 KB in all
   static constexpr int kRing = kStages * kStage;
   static constexpr int kDescribed = kWarps * 32 * 16;  // 32 tiles of a warp
-  static constexpr int kSmem = kWarps * kRing + kDescribed;
+  // An A operand is four registers in a row: with up to 8 query heads half of them are zeros, 64 registers in all at
+  // head_dim 256, which spills (64 x 2000 tokens, 16 / 8 heads: 198 - 219 us).  There the queries stand in shared
+  // memory, and a chunk of zeros for the other rows (168 us).
+  static constexpr bool kQueries = D == 256 && !R16;
+  static constexpr int kQuery = 8 * kRow;
+  static constexpr int kZeros = kWarps * kRing + kDescribed + kWarps * kQuery;
+  static constexpr int kSmem = kQueries ? kZeros + 16 : kWarps * kRing + kDescribed;
   // The 16-byte chunks of a row are permuted, so that the same chunk of 8 rows stands in all banks.
   static __device__ __forceinline__ int key(int row) { return D == 96 ? row >> 1 & 3 : row & 7; }
 };
@@ -150,12 +156,13 @@ __device__ __forceinline__ float dense_lse(float m, float l, float lift) {
 }
 
 template <typename T, int D, bool R16>
-__global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_kernel(const DenseArgs p) {
-  using S = DenseShape<D>;
+__global__ void __launch_bounds__(DenseShape<D, R16>::kWarps * 32, 1) dense_decode_kernel(const DenseArgs p) {
+  using S = DenseShape<D, R16>;
   using X = Dense16<T>;
   constexpr int kSteps = D / 16, kBlocks = D / 8;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int warp_total[S::kWarps];
+  __shared__ DenseCut cut;  // (ten registers less, where head_dim 256 has none to spare)
   int4* const described = reinterpret_cast<int4*>(smem + S::kWarps * S::kRing);
   int* const prefix = reinterpret_cast<int*>(smem + S::kSmem);  // [seqs + 1]
   int* const lengths = prefix + p.seqs + 1;                     // [seqs]
@@ -164,6 +171,7 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
   const int g = lane >> 2, t = lane & 3;
   const int64_t room = int64_t(p.table_width) * p.block_size;
   const int unit_groups = p.unit_groups;
+  if (S::kQueries && tid < 4) reinterpret_cast<uint32_t*>(smem + S::kZeros)[tid] = 0u;
   // (the wait first: the second kernel, which this lets start, reads what the kernels before this one have written)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -197,10 +205,10 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
       if (blockIdx.x == 0) p.bounds[s + 1] = prefix[s + 1];
     }
     if (blockIdx.x == 0 && tid == 0) p.bounds[0] = 0;
+    if (tid == S::kWarps * 32 - 1) cut = dense_cut(before + sum, p.fixed, p.seqs * unit_groups);
     __syncthreads();
   }
   const int groups_all = p.seqs * unit_groups;
-  const DenseCut cut = dense_cut(prefix[p.seqs], p.fixed, groups_all);
 
   // ---- the warp's tiles, described sixteen at a time ---------------------------------------------------
   const int tiles_per_block = p.block_size / kDenseTile;
@@ -292,32 +300,57 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
       const T* v = static_cast<const T*>(p.v) + id * p.v_block + row * p.v_token + head * p.v_head;
       const int lo = (d.y >> 22) & 15, hi = d.x < 0 ? 0 : (d.y >> 26) & 31;
       const uint32_t dst = ring + stage * S::kStage;
+      // (the rows of a tile stand in one page: those outside the sequence have an address, and nothing is read there)
+      const int r0 = lane / kPerRow, col = lane % kPerRow;
+      const T *ks = k + r0 * p.k_token + col * 8, *vs = v + r0 * p.v_token + col * 8;
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
-        const int i = lane + 32 * c, r = i / kPerRow, col = i % kPerRow;
-        const bool valid = r >= lo && r < hi;
-        const uint32_t to = dst + r * S::kRow + ((col ^ S::key(r)) << 4);
-        cp_async16(to, k + (valid ? r * p.k_token + col * 8 : 0), valid, policy);
-        cp_async16(to + S::kTensor, v + (valid ? r * p.v_token + col * 8 : 0), valid, policy);
+        if constexpr (32 % kPerRow == 0) {
+          constexpr int kRows = 32 / kPerRow;
+          const int r = r0 + c * kRows;
+          const bool valid = r >= lo && r < hi;
+          const uint32_t to = dst + r * S::kRow + ((col ^ S::key(r)) << 4);
+          cp_async16(to, ks, valid, policy);
+          cp_async16(to + S::kTensor, vs, valid, policy);
+          ks += kRows * p.k_token;
+          vs += kRows * p.v_token;
+        } else {
+          const int i = lane + 32 * c, r = i / kPerRow, at = i % kPerRow;
+          const bool valid = r >= lo && r < hi;
+          const uint32_t to = dst + r * S::kRow + ((at ^ S::key(r)) << 4);
+          cp_async16(to, k + r * p.k_token + at * 8, valid, policy);
+          cp_async16(to + S::kTensor, v + r * p.v_token + at * 8, valid, policy);
+        }
       }
     }
     cp_async_commit();
   };
 
   // ---- state of the unit in work ----------------------------------------------------------------------
-  uint32_t qf[kSteps][R16 ? 4 : 2];
+  uint32_t qf[S::kQueries ? 1 : kSteps][R16 ? 4 : 2];
+  unsigned char* const queries = smem + S::kWarps * S::kRing + S::kDescribed + warp * S::kQuery;  // (kQueries)
   float acc[kBlocks][4];
   float top[R16 ? 2 : 1], sum[R16 ? 2 : 1];
 
   auto begin_unit = [&](const int4& d) {
     const DenseUnit u = dense_unit(p, (d.z >> 12) & 0x3fff);
     const T* q = static_cast<const T*>(p.q) + (d.z & 0xfff) * p.q_seq + u.head0 * p.q_head;
+    if constexpr (S::kQueries) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+          const int word = lane + 32 * i;  // of the row
+          const uint32_t x = r < u.count ? *reinterpret_cast<const uint32_t*>(q + r * p.q_head + 2 * word) : 0u;
+          *reinterpret_cast<uint32_t*>(queries + r * S::kRow + ((word / 4 ^ S::key(r)) << 4) + word % 4 * 4) = x;
+        }
+    }
 #pragma unroll
     for (int r = 0; r < (R16 ? 2 : 1); ++r) {
       const bool real = g + 8 * r < u.count;
       const T* row = q + (real ? (g + 8 * r) * p.q_head : 0) + 2 * t;
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
+      for (int s = 0; s < (S::kQueries ? 0 : kSteps); ++s) {
         const uint32_t x = *reinterpret_cast<const uint32_t*>(row + 16 * s);
         const uint32_t y = *reinterpret_cast<const uint32_t*>(row + 16 * s + 8);
         qf[s][r] = real ? x : 0u;
@@ -336,13 +369,18 @@ __global__ void __launch_bounds__(DenseShape<D>::kWarps * 32, 1) dense_decode_ke
     // scores: rows = heads, columns = tokens (two blocks of eight)
     float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
     const int k_row = (mid >> 1) * 8 + (lane & 7), v_row = (mid & 1) * 8 + (lane & 7);
+    // (kQueries) rows 0 - 7 for the lanes of the first and third matrix, zeros for the others
+    const uint32_t q_real = ~mid & 1, q_key = ((mid >> 1) ^ S::key(lane & 7)) << 4;
+    const uint32_t qa = q_real ? smem_u32(queries) + (lane & 7) * S::kRow : smem_u32(smem + S::kZeros);
     const uint32_t ka = kt + k_row * S::kRow, k_key = ((mid & 1) ^ S::key(k_row)) << 4;
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
       uint32_t b[4];
       ldmatrix4(b, ka + (i * 32 ^ k_key));
       uint32_t a[4];
-      if constexpr (R16) {
+      if constexpr (S::kQueries) {
+        ldmatrix4(a, qa + (i * 32 ^ q_key) * q_real);
+      } else if constexpr (R16) {
         a[0] = qf[i][0]; a[1] = qf[i][1]; a[2] = qf[i][2]; a[3] = qf[i][3];
       } else {
         a[0] = qf[i][0]; a[1] = 0u; a[2] = qf[i][1]; a[3] = 0u;
@@ -750,7 +788,7 @@ static int launch_join(DenseArgs p, cudaStream_t stream) {
 
 template <typename T, int D, bool R16>
 static int launch_dense(const DenseArgs& p, int ctas, cudaStream_t stream) {
-  using S = DenseShape<D>;
+  using S = DenseShape<D, R16>;
   const size_t smem = S::kSmem + (2 * size_t(p.seqs) + 1) * sizeof(int);
   const auto kernel = dense_decode_kernel<T, D, R16>;
   static thread_local DenseDevice known;
