@@ -703,7 +703,8 @@ struct DenseGeometry {
   int chunks, rows, group, side_bits, piece_floats;
   bool r16;
 };
-// Up to 8 query heads to a unit (16 where a KV head has more: its keys are then read half as often).
+// Up to 8 query heads to a unit, 16 where a KV head has more: its keys are then read half as often (64 x 4000 tokens, 20 / 2
+// heads: 70 us with units of 8, 55 with 16; 32 / 2: 71, 55).
 static DenseGeometry dense_geometry(int hq, int hkv, int d) {
   DenseGeometry x;
   x.group = hq / hkv;
@@ -760,29 +761,35 @@ static int launch_dependent(void (*kernel)(DenseArgs), const DenseArgs& p, dim3 
   return check_launch("dense decode");
 }
 
-// As many heads to a CTA of the join as leave it with eight CTAs on an SM, all resident at once; where there are few
-// heads, their dimensions are split, and the pieces of a unit where it can have hundreds (1 x 131072 tokens, 8 query
-// heads on one KV head: 55 us the call without, 27 with).
+// As few heads to a CTA of the join as leave it with eight CTAs on an SM, all resident at once.  Where that leaves room, the
+// pieces of a unit are split over a cluster, 64 or fewer to a CTA (1 x 131072 tokens, 8 query heads on one KV head: 55 us the
+// call without, 25 with), and the dimensions of a head where it still has more than 24 (1 x 900: 13.7 us with whole
+// heads, 10.1 with 32 dimensions; 1 x 32768: 35.9 with the dimensions split first, 32.4 like this).
 template <typename T, int D>
 static int launch_join(DenseArgs p, cudaStream_t stream) {
   const int64_t units = int64_t(p.seqs) * p.hkv * p.chunks, most = 8 * kDenseMaxCtas;
+  const int64_t tiles = int64_t(p.table_width) * (p.block_size / kDenseTile);
+  const int64_t pieces = std::min(tiles, (int64_t(p.fixed) << p.side_bits) / units + 1);  // of a unit, about
   p.join_rows = 1;
   p.join_wide = D;
-  if (units * p.rows * (D / 32) <= most) p.join_wide = 32;
-  else if (D % 64 == 0 && units * p.rows * (D / 64) <= most) p.join_wide = 64;
-  const auto ctas = [&] { return units * ((p.rows + p.join_rows - 1) / p.join_rows) * (D / p.join_wide); };
+  p.join_split = 1;
+  const auto ctas = [&] {
+    return units * ((p.rows + p.join_rows - 1) / p.join_rows) * (D / p.join_wide) * p.join_split;
+  };
   while (p.join_rows < p.rows && 2 * p.join_rows <= kJoinRows && 2 * p.join_rows * p.join_wide / 4 <= kJoinThreads &&
          ctas() > most)
     p.join_rows *= 2;
+  while (p.join_split < 8 && pieces > 64 * p.join_split && 2 * ctas() <= most) p.join_split *= 2;
+  if (pieces > 24 * p.join_split) {
+    if (ctas() * (D / 32) <= most) p.join_wide = 32;
+    else if (D % 64 == 0 && ctas() * (D / 64) <= most) p.join_wide = 64;
+  }
   p.join_wides = D / p.join_wide;
   p.join_columns = p.join_rows * p.join_wide / 4;
   p.join_groups = kJoinThreads / p.join_columns;
-  const int64_t tiles = int64_t(p.table_width) * (p.block_size / kDenseTile);
-  const int64_t pieces = std::min(tiles, (int64_t(p.fixed) * (1 + kDenseTaken) << p.side_bits) / units);  // of a unit, about
-  p.join_split = 1;
-  while (p.join_split < 8 && pieces > 64 * p.join_split && 2 * p.join_split * ctas() <= most) p.join_split *= 2;
-  const int64_t over = (ctas() + most - 1) / most;  // units of a sequence that a CTA takes
-  const dim3 grid(unsigned((p.hkv * p.chunks + over - 1) / over), (p.rows + p.join_rows - 1) / p.join_rows * p.join_wides, p.seqs * p.join_split);
+  const int64_t over = (ctas() + most - 1) / most;  // units of a sequence that a CTA takes (1 where there is a split)
+  const dim3 grid(unsigned((p.hkv * p.chunks + over - 1) / over),
+                  (p.rows + p.join_rows - 1) / p.join_rows * p.join_wides, p.seqs * p.join_split);
   return launch_dependent(dense_join_kernel<T, D>, p, grid, kJoinThreads, 0, p.join_split, stream);
 }
 

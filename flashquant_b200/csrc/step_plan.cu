@@ -283,6 +283,7 @@ __global__ void __launch_bounds__(kPlanThreads) release_pages_kernel(const Relea
   if (cta == 0 && tid == 0) *p.count_out = int32_t(height + total);
 }
 
+// (64 prompts, 39 000 tokens: 10.2 us by a cluster of eight CTAs, 5.5 by one to 1024; 128 000 pages released: 15.3, 4.4)
 constexpr int kPlanCluster = 8, kPlanMaxCtas = 148;
 // `work`: pages or tokens
 template <typename Args>

@@ -329,6 +329,28 @@ def test_recorded_behind_a_fork():
         graph.reset()
 
 
+def test_recorded_clusters_and_long_prompts():
+    """Pieces joined by clusters, and rotary positions of a prompt, in a recorded graph."""
+    b = Batch([60000, 2, 9000], 8, 1, 128, HF)
+    want = b.call()
+    b.check(want)
+    q, k = heads(3000, (8, 1), 128, HF, joint=True)
+    freq, _ = fq.rotary_frequencies(128, device=DEV)
+    pos = torch.randint(0, 9000, (3000,), device=DEV)
+    turned_q, turned_k = fq.rotary_embed(q, k, pos, freq)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x, y = fq.rotary_embed(q, k, pos, freq)
+        out = b.call()
+    for _ in range(5):
+        out.zero_(), x.zero_(), y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(x, turned_q) and torch.equal(y, turned_k)
+    graph.reset()
+
+
 def test_what_follows_waits_for_all_of_a_decode():
     """A batch of which no unit has to be joined, long enough to be under way when what follows it is launched:
     eager and recorded, the reader of its output sees all of it."""
@@ -536,7 +558,7 @@ def test_rotary_inverse_is_the_gradient():
         step = torch.randn_like(y)  # linear: one difference is exact but for its rounding in 64 bits
         f = lambda z: (turned(z, pos, freq, layout, 1.5)[0] * g.double()).sum()
         diff = f(y + step) - f(y - step)
-        assert abs(float(diff) / 2 - float((back.double() * step).sum())) <= float((tol * step.abs()).sum()) + 1e-9
+        assert abs(float(diff.detach()) / 2 - float((back.double() * step).sum())) <= float((tol * step.abs()).sum()) + 1e-9
 
 
 def test_rotary_refusals():
