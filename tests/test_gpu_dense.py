@@ -476,7 +476,7 @@ def heads(n, h, d, dtype, seed=0, joint=False):
 @pytest.mark.parametrize("dtype", [torch.float32, BF, HF])
 @pytest.mark.parametrize("layout", ["half", "interleaved"])
 @pytest.mark.parametrize("d, rd", [(128, 128), (128, 64), (64, 64), (96, 96), (80, 32), (96, 24), (256, 128), (128, 2), (6, 4),
-                                   (128, 0)])
+                                   (128, 0), (5, 4), (7, 0), (9, 6), (1024, 512)])
 def test_rotary(dtype, layout, d, rd):
     n = 37
     q, k = heads(n, (6, 2), d, dtype, seed=d + rd, joint=d == 96)
