@@ -402,7 +402,8 @@ __global__ void __launch_bounds__(DenseShape<D, R16>::kWarps * 32, 1) dense_deco
           if (at < lo || at >= hi) s[n][e] = -INFINITY;
         }
     }
-    uint32_t hi_a[4], lo_a[4];
+    uint32_t hi_a[4];
+    [[maybe_unused]] uint32_t lo_a[4];
 #pragma unroll
     for (int r = 0; r < (R16 ? 2 : 1); ++r) {
       float m = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
