@@ -521,18 +521,16 @@ __global__ void __launch_bounds__(DenseShape<D, R16>::kWarps * 32, 1) dense_deco
   cp_async_wait<0>();
 }
 
-// A cluster for `join_rows` query heads of a unit, or of a few units one after the other, and `join_wide` of their dimensions, each of its CTAs for a part of the
-// pieces: their weights first, a warp to a head and a lane to a piece, then the sums, a group of threads to a piece, and
-// the first CTA adds up what the others have in their shared memory.  A unit that one run had is left alone; heads without
-// tokens get zeros.  What does not depend on the pieces is done before the wait for the first kernel, and the first pieces
-// are on their way with the weights.  No CTA leaves before that wait: the kernel must not end before the first one has.
+// A cluster for `join_rows` query heads of a unit, or of a few units one after the other, and `join_wide` of their
+// dimensions, each of its CTAs for a part of the pieces: their weights first, a warp to a head and a lane to a piece, then
+// the sums, a group of threads to a piece, and the first CTA adds up what the others have in their shared memory.  A unit
+// that one run had is left alone; heads without tokens get zeros.  The first pieces are on their way with the weights.
 constexpr int kJoinThreads = 128, kJoinPieces = 128, kJoinRows = 4;
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const DenseArgs p) {
-  constexpr int kAhead = 4, kWarps = kJoinThreads / 32;
+  constexpr int kAhead = 4;
   __shared__ float weights[kJoinRows][kJoinPieces];
   __shared__ float totals[kJoinRows][3];  // maximum, sum, factor of what stands
-  __shared__ int counts[kWarps][2];
   __shared__ float4 sums[kJoinThreads];
   const cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -543,38 +541,12 @@ __global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const Dense
   const int mine = tid / columns, column = tid - mine * columns;
   const int row = column * 4 / p.join_wide;
   const int dim = wide * p.join_wide + column * 4 - row * p.join_wide;
-  int s0, tiles, total;
-  if (p.seqs <= 4 * kJoinThreads) {
-    const int64_t room = int64_t(p.table_width) * p.block_size;
-    tiles = dense_span(p.lens[seq], room, p.window).tiles;
-    int all = 0, before = 0;
-    for (int s = tid; s < p.seqs; s += kJoinThreads) {
-      const int own = dense_span(p.lens[s], room, p.window).tiles;
-      all += own;
-      if (s < seq) before += own;
-    }
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) {
-      all += __shfl_xor_sync(0xffffffffu, all, s);
-      before += __shfl_xor_sync(0xffffffffu, before, s);
-    }
-    if (lane == 0) {
-      counts[warp][0] = all;
-      counts[warp][1] = before;
-    }
-    __syncthreads();
-    total = s0 = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      total += counts[w][0] * unit_groups;
-      s0 += counts[w][1] * unit_groups;
-    }
-  } else {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    s0 = p.bounds[seq];
-    tiles = (p.bounds[seq + 1] - s0) / unit_groups;
-    total = p.bounds[p.seqs];
-  }
+  // Nothing that another kernel has written is read before this wait, the lengths neither: the first kernel has waited for
+  // what came before it, but what a kernel sees is promised behind a wait of its own only.  No CTA leaves before it: this
+  // kernel must not end before the first one has.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int s0 = p.bounds[seq], tiles = (p.bounds[seq + 1] - s0) / unit_groups, total = p.bounds[p.seqs];
   const bool with_lse = p.lse && wide == 0 && part == 0;
   const int groups_all = p.seqs * unit_groups;
   const DenseCut cut = dense_cut(total, p.fixed, groups_all);
@@ -593,8 +565,6 @@ __global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const Dense
     const int a = s0 + group * tiles;
     const DensePieces all = dense_pieces(cut, a, a + tiles);
     const int pieces = all.count(), first = pieces * part / parts, n = pieces * (part + 1) / parts;
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // (passed at once from the second unit on)
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (tiles == 0 && part == 0) {
       if (real && mine == 0) write(make_float4(0.f, 0.f, 0.f, 0.f));
       if (with_lse && tid < rows) p.lse[out_row + tid] = -INFINITY;

@@ -1,0 +1,48 @@
+"""Calls around 16-bit pages that a program may make and the other tests do not: tolerances are those of
+test_gpu_dense.py, most comparisons are of bits."""
+
+import threading
+
+import pytest
+import torch
+
+import flashquant_b200 as fq
+from flashquant_b200 import _native as N
+from flashquant_b200 import kernels as K
+from test_gpu_dense import BF, DEV, HF, Batch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("recorded", [False, True])
+@pytest.mark.parametrize("seqs", [3, 700])
+def test_lengths_written_right_before_the_call(seqs, recorded):
+    """Both kernels of a decode go by the lengths that the kernel before the call has written, not by older ones."""
+    g = torch.Generator().manual_seed(seqs)
+    longest = 6000 if seqs == 3 else 90
+    b = Batch([longest] * seqs, 32, 8, 128, BF, spare=0)
+    lens = torch.randint(0, longest + 1, (12, seqs), generator=g).int().to(DEV)
+    want = []
+    for n in lens:
+        b.sl.copy_(n)
+        torch.cuda.synchronize()
+        want.append(b.call(return_lse=True))
+        torch.cuda.synchronize()
+    source = torch.empty_like(b.sl)
+    copied = lambda: (b.sl.copy_(source), b.call(return_lse=True))[1]
+    graph = None
+    if recorded:
+        source.copy_(lens[0])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            made = copied()
+    for step in range(60):
+        source.copy_(lens[step % 12])
+        if recorded:
+            graph.replay()
+        else:
+            made = copied()
+        for x, w in zip(made, want[step % 12]):
+            assert torch.equal(x, w)
+    if graph is not None:
+        graph.reset()
