@@ -724,15 +724,14 @@ PyObject* dense_decode(PyObject*, Args a, Py_ssize_t n) {
   // counters when they run side by side.
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
   if (cudaStreamIsCapturing(reinterpret_cast<cudaStream_t>(stream_of(dev)), &capture) != cudaSuccess) return none();
-  std::mutex* calls = nullptr;
   Tensor ws;
   if (capture == cudaStreamCaptureStatusNone) {
-    ws = workspace(dev, kDense, need, &calls);
+    ws = workspace(dev, kDense, need);
   } else {
     ws = call_bytes(dev, need, false);
     ws.narrow(0, 0, 32768).zero_();
   }
-  const int rc = native(calls, [&] {
+  const int rc = native(nullptr, [&] {  // (the entry has a lock of its own, for callers of every path)
     return fq_dense_paged_decode(
         q->data_ptr(), fq_dtype(dtype_code(*q)), q->stride(0), q->stride(1), kc->data_ptr(), kc->stride(0),
         kc->stride(1), kc->stride(2), vc->data_ptr(), vc->stride(0), vc->stride(1), vc->stride(2),

@@ -46,3 +46,28 @@ def test_lengths_written_right_before_the_call(seqs, recorded):
             assert torch.equal(x, w)
     if graph is not None:
         graph.reset()
+
+
+@pytest.mark.parametrize("paths", ["both converted", "one converted"])
+def test_decodes_of_converted_arguments_from_two_threads(monkeypatch, paths):
+    """Calls whose arguments are converted (a whole number for the scale, lengths a column of a table) share the stream's
+    workspace with those of other threads like all others."""
+    a, b = Batch([4000, 9, 1300], 32, 8, 128, BF), Batch([2, 5000, 77], 32, 8, 128, BF, seed=5)
+    b.sl = torch.stack([b.sl, b.sl], 1)[:, 0]
+    want = a.call(sm_scale=1.0), b.call()
+    torch.cuda.synchronize()
+    if paths == "both converted":
+        monkeypatch.setattr(K, "_host_module", K._ConvertingCalls())
+    wrong = []
+
+    def work(x, w, kw):
+        outs = [x.call(**kw) for _ in range(300)]
+        torch.cuda.synchronize()
+        wrong.extend(o for o in outs if not torch.equal(o, w))
+    threads = [threading.Thread(target=work, args=z)
+               for z in zip((a, b), want, (dict(sm_scale=1 if paths == "both converted" else 1.0), {}))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
