@@ -395,6 +395,8 @@ def split_k_paged_decode_dense(q, key_cache, value_cache, block_table, seq_lens,
         raise ValueError("all tensors must be on one device")
     if window < 0:
         raise ValueError("window must not be negative")
+    if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous()):
+        raise ValueError("workspace must be a contiguous uint8 tensor")  # (its numel is taken for its bytes)
     if q.stride(2) != 1 or q.stride(0) % 2 or q.stride(1) % 2 or q.data_ptr() % 4:
         q = q.clone(memory_format=torch.contiguous_format)
     if block_table.shape[1] > 1 and block_table.stride(1) != 1:

@@ -5,7 +5,10 @@ import os
 import re
 
 import pytest
+import torch
 
+import flashquant_b200 as fq
+from flashquant_b200 import _native as N
 from conftest import ROOT
 
 CSRC = os.path.join(ROOT, "flashquant_b200", "csrc")
@@ -34,3 +37,18 @@ def test_nothing_is_read_before_the_wait(name):
     assert {"q", "k", "v", "out", "lse", "table", "lens", "status", "tickets", "bounds", "pieces"} <= set(pointers)
     for n in pointers:
         assert not re.search(r"\bp\.%s\b" % n, before), n
+
+
+def _decode_args(**kw):
+    pages = torch.zeros(4, 16, 8, 128, dtype=torch.float16)
+    return {**dict(q=torch.zeros(2, 8, 128, dtype=torch.float16), key_cache=pages, value_cache=pages,
+                   block_table=torch.zeros(2, 2, dtype=torch.int32), seq_lens=torch.ones(2, dtype=torch.int32)), **kw}
+
+
+@pytest.mark.parametrize("workspace", [torch.zeros(1, dtype=torch.uint8).expand(1 << 28), torch.zeros(1 << 12, dtype=torch.uint8)[::2],
+                                       torch.zeros(1 << 12), torch.zeros(64, 64, dtype=torch.uint8).t()])
+def test_workspaces_that_are_not_plain_bytes(monkeypatch, workspace):
+    """A workspace whose number of values is not the number of bytes behind its address is refused before anything else."""
+    monkeypatch.setattr(N, "require_cuda", lambda *t: None)
+    with pytest.raises(ValueError, match="workspace"):
+        fq.split_k_paged_decode_dense(**_decode_args(workspace=workspace))
