@@ -21,6 +21,7 @@ from .kernels import _DENSE, _contig, _host, _workspace
 _HEAD = 32768  # bytes at the start of a decode workspace that are zero between calls
 _LAYOUTS = {"half": 0, "interleaved": 1}
 _INTS = (torch.int32, torch.int64)
+_MOST = 2 ** 31 - 1  # (ctypes keeps the low bits of a larger int)
 
 
 def _layout(name: str) -> int:
@@ -87,8 +88,8 @@ def plan_paged_step(context_lens, query_lens, block_table, free_blocks, free_cou
     N.require_cuda(context_lens, query_lens)
     _pool_args(block_table, free_blocks, free_count, free_count_out)
     dev, (n, width) = block_table.device, block_table.shape
-    if max_tokens < 0 or block_size < 1:
-        raise ValueError("max_tokens must not be negative, block_size positive")
+    if max_tokens < 0 or not 1 <= block_size <= _MOST:
+        raise ValueError("max_tokens must not be negative, block_size positive and below 2^31")
     context, query = (_lens(t, n, dev, m) for t, m in ((context_lens, "context_lens"), (query_lens, "query_lens")))
     i32 = dict(dtype=torch.int32, device=dev)
     plan = PagedStepPlan(torch.empty(n, **i32), torch.empty(n + 1, **i32),
@@ -120,8 +121,8 @@ def release_pages(finished, context_lens, block_table, free_blocks, free_count, 
     dev, (n, width) = block_table.device, block_table.shape
     if finished.dim() != 1 or finished.shape[0] != n or finished.dtype != torch.bool:
         raise ValueError("finished must hold one bool per row of block_table")
-    if block_size < 1:
-        raise ValueError("block_size must be positive")
+    if not 1 <= block_size <= _MOST:
+        raise ValueError("block_size must be positive and below 2^31")
     context, finished = _lens(context_lens, n, dev, "context_lens"), _contig(finished.to(dev))
     out = torch.empty(1, dtype=torch.int32, device=dev) if free_count_out is None else free_count_out
     with torch.cuda.device(dev):
@@ -418,6 +419,7 @@ def split_k_paged_decode_dense(q, key_cache, value_cache, block_table, seq_lens,
         N.check(lib.fq_dense_paged_decode(
             N.ptr(q), N.dtype_code(q.dtype), q.stride(0), q.stride(1), N.ptr(key_cache), *key_cache.stride()[:3],
             N.ptr(value_cache), *value_cache.stride()[:3], N.ptr(block_table), block_table.stride(0),
-            block_table.shape[1], N.ptr(seq_lens), n, hq, hkv, d, bs, blocks, float(sm_scale), int(window), N.ptr(out),
+            block_table.shape[1], N.ptr(seq_lens), n, hq, hkv, d, bs, blocks, float(sm_scale),
+            min(int(window), _MOST), N.ptr(out),
             N.ptr(lse), N.ptr(workspace), workspace.numel(), N.stream_ptr(dev)))
     return (out, lse) if return_lse else out

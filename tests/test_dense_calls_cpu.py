@@ -52,3 +52,13 @@ def test_workspaces_that_are_not_plain_bytes(monkeypatch, workspace):
     monkeypatch.setattr(N, "require_cuda", lambda *t: None)
     with pytest.raises(ValueError, match="workspace"):
         fq.split_k_paged_decode_dense(**_decode_args(workspace=workspace))
+
+
+@pytest.mark.parametrize("block_size", [2 ** 32 + 16, 2 ** 31, 2 ** 64 + 1, 0, -16])
+def test_block_sizes_beyond_32_bits(monkeypatch, block_size):
+    monkeypatch.setattr(N, "require_cuda", lambda *t: None)
+    i32 = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="block_size"):
+        fq.plan_paged_step(i32, i32, i32.view(2, 1), i32, i32[:1], block_size, 8)
+    with pytest.raises(ValueError, match="block_size"):
+        fq.release_pages(i32.bool(), i32, i32.view(2, 1), i32, i32[:1], block_size)

@@ -71,3 +71,11 @@ def test_decodes_of_converted_arguments_from_two_threads(monkeypatch, paths):
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 5, 2 ** 63])
+def test_windows_beyond_32_bits_see_all(window):
+    b = Batch([40, 700, 9], 32, 8, 128, BF)
+    want = b.call()
+    b.window = window
+    assert torch.equal(b.call(), want)
