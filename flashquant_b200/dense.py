@@ -64,6 +64,8 @@ def _pool_args(block_table, free_blocks, free_count, free_count_out):
 def _lens(t, n, device, name):
     if t.dim() != 1 or t.shape[0] != n or t.dtype not in _INTS:
         raise ValueError(f"{name} must hold one int32 or int64 per row of block_table")
+    if t.dtype == torch.int64:  # what does not fit stays too long, or negative
+        t = t.clamp(-1, _MOST)
     return _contig(t.to(device=device, dtype=torch.int32))
 
 

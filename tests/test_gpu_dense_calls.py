@@ -79,3 +79,22 @@ def test_windows_beyond_32_bits_see_all(window):
     want = b.call()
     b.window = window
     assert torch.equal(b.call(), want)
+
+
+I32 = dict(dtype=torch.int32, device=DEV)
+
+
+def test_lengths_beyond_32_bits_are_too_long():
+    """64-bit lengths that do not fit into 32 bits: more pages than a row holds (or negative), not what their low bits say."""
+    table = torch.tensor([[3, 4], [5, 6], [7, 8], [9, 10], [11, 12]], **I32)
+    context = torch.tensor([2 ** 32 + 3, 0, -2 ** 32 + 3, 2, 2 ** 31 + 1], device=DEV)
+    query = torch.tensor([1, 2 ** 32 + 1, 1, 1, 0], device=DEV)
+    free, height = torch.arange(50, 60, **I32), torch.tensor([10], **I32)
+    plan = fq.plan_paged_step(context, query, table.clone(), free, height, 16, 8)
+    assert plan.served.tolist() == [False, False, False, True, False]
+    assert plan.cu_seqlens_q.tolist() == [0, 0, 0, 0, 1, 1] and plan.slot_mapping.tolist() == [9 * 16 + 2] + [-1] * 7
+    assert plan.seq_lens.tolist() == [32, 0, 0, 3, 32] and int(plan.free_count) == 10
+    done = torch.ones(5, dtype=torch.bool, device=DEV)
+    stack = torch.full((20,), -1, **I32)
+    out = fq.release_pages(done, context, table, stack, torch.zeros(1, **I32), 16)
+    assert int(out) == 5 and stack[:5].tolist() == [3, 4, 9, 11, 12]
