@@ -140,7 +140,7 @@ def release_pages(finished, context_lens, block_table, free_blocks, free_count, 
 # --------------------------------------------------------------------------------------
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0,
-                       original_length: int = 8192, low: float = 1.0, high: float = 4.0,
+                       original_length: int = 8192, low: float = 1.0, high: Optional[float] = None,
                        device=None) -> Tuple[torch.Tensor, float]:
     """``(frequencies, scale)`` for the rotary entry points: ``rotary_dim / 2`` angles per position in
     fp64, ``base ** (-2j / rotary_dim)``, and what rotated values are multiplied with.
@@ -150,11 +150,14 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
       "linear"      all divided by ``factor``
       "ntk"         another base, ``base * factor ** (rotary_dim / (rotary_dim - 2))``: the slowest is
                     divided by ``factor``, the fastest kept
-      "wavelength"  kept where ``original_length`` holds ``high`` or more turns, divided where it holds
+      "wavelength"  kept where ``original_length`` holds ``high`` (4) or more turns, divided where it holds
                     ``low`` or fewer, blended by the number of turns between
-      "yarn"        the same blended linearly over the index, between those that make ``high`` (commonly
-                    32) and ``low`` turns; values are multiplied by ``0.1 ln factor + 1``
+      "yarn"        the same blended linearly over the index, between those that make ``high`` (32) and ``low``
+                    turns, the latter at most ``rotary_dim - 1``: it may lie behind the last frequency, which is
+                    then not fully divided; values are multiplied by ``0.1 ln factor + 1``
     """
+    if high is None:
+        high = 32.0 if scaling == "yarn" else 4.0
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
     if not (base > 1.0 and factor >= 1.0 and original_length > 0 and 0 < low < high):
@@ -176,7 +179,7 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
         else:
             def index(n):  # of the frequency that makes n turns
                 return half * math.log(original_length / (n * 2.0 * math.pi)) / math.log(base)
-            first, last = max(math.floor(index(high)), 0), min(math.ceil(index(low)), half - 1)
+            first, last = max(math.floor(index(high)), 0), min(math.ceil(index(low)), rotary_dim - 1)
             keep = 1.0 - ((j - first) / max(last - first, 1e-3)).clamp(0, 1)
             scale = 0.1 * math.log(factor) + 1.0
         freq = freq * keep + freq / factor * (1.0 - keep)
