@@ -81,7 +81,11 @@ def plan_paged_step(context_lens, query_lens, block_table, free_blocks, free_cou
 
     A request is served if the pages and slots of all requests up to and including it can be had, or if
     it has no new tokens; from the first that is not, only those without new tokens are.  A negative
-    length, or more pages than a row holds, is not served and takes nothing.
+    length, or more pages than a row holds, is not served and takes nothing.  At most 4096 requests.
+
+    The tokens' rows are compact, request ``i``'s from ``cu_seqlens_q[i]`` on: the decodes, which take a row of
+    ``q`` per row of ``block_table``, are given ``q[cu_seqlens_q[:-1]]`` (cut to ``max_tokens - 1``), unless every
+    request is known to be served with one token.
     """
     r = _host().plan_paged_step(context_lens, query_lens, block_table, free_blocks, free_count, block_size,
                                 max_tokens, free_count_out)

@@ -98,3 +98,76 @@ def test_lengths_beyond_32_bits_are_too_long():
     stack = torch.full((20,), -1, **I32)
     out = fq.release_pages(done, context, table, stack, torch.zeros(1, **I32), 16)
     assert int(out) == 5 and stack[:5].tolist() == [3, 4, 9, 11, 12]
+
+
+@pytest.mark.parametrize("recorded", [False, True])
+def test_a_step_that_not_every_request_takes_part_in(consts, recorded):
+    """Requests that are finished, wait or are not served stand between others: rows of tokens are compact, those of the
+    decodes are not.  Each token's row is that of its request in a call whose rows a list has put in their places."""
+    r, hq, hkv, d, block, width, room = 7, 32, 8, 128, 16, 8, 5
+    g = torch.Generator(device=DEV).manual_seed(4)
+    rot, bk, bv, ck, cv = (consts[x].contiguous().to(DEV) for x in (
+        "rotation_128_0", "boundaries_128_3", "boundaries_128_4", "centroids_128_3", "centroids_128_4"))
+    blocks = 64
+    kc, vc = (torch.randn(blocks, block, hkv, d, generator=g, device=DEV).to(BF) for _ in range(2))
+    packed = torch.zeros(blocks, block, hkv * (d + 8), dtype=torch.uint8, device=DEV)
+    every = torch.arange(blocks * block, device=DEV)
+    fq.tq4_compress_append(kc.view(-1, hkv, d), vc.view(-1, hkv, d), packed, every, rot, bk, bv)
+    table0 = torch.randperm(blocks, generator=g, device=DEV).int()[:r * width].view(r, width).contiguous()
+    free = torch.arange(56, 64, **I32)
+    freq, scale = fq.rotary_frequencies(d, device=DEV)
+    context, query, height, table = torch.zeros(r, **I32), torch.zeros(r, **I32), torch.zeros(1, **I32), table0.clone()
+    qkv = torch.randn(room, hq + 2 * hkv, d, generator=g, device=DEV).to(BF)
+    tokens = torch.arange(room, **I32)
+
+    def step():
+        plan = fq.plan_paged_step(context, query, table, free, height, block, room, free_count_out=height)
+        first = plan.cu_seqlens_q[:-1].clamp(max=room - 1)
+        owner = torch.searchsorted(plan.cu_seqlens_q[1:], tokens, right=True).clamp(max=r - 1)
+        q, k, v = torch.split(qkv, (hq, hkv, hkv), 1)
+        rq, rk = fq.rotary_embed(q, k, plan.positions, freq, scale=scale)
+        fq.tq4_compress_append(rk, v, packed, plan.slot_mapping, rot, bk, bv)
+        out4 = fq.split_k_paged_decode(rq[first], packed, table, plan.seq_lens, ck, cv, rot, hkv, d, block)[owner]
+        q = fq.rotary_append_dense(q, k, v, kc, vc, plan.slot_mapping, plan.positions, freq, scale=scale)
+        out = fq.split_k_paged_decode_dense(q[first], kc, vc, table, plan.seq_lens)[owner]
+        return plan, q, out4, out
+
+    # contexts, new tokens, pages left; who is served with a token
+    cases = [([5, 17, 40, 3, 90, 60, 33], [0, 1, 0, 1, 1, 0, 1], 8, [1, 3, 4, 6]),
+             ([5, 16, 40, 3, 96, 60, 33], [1, 1, 0, 1, 1, 0, 1], 1, [0, 1, 3]),   # no page for the fifth
+             ([5, 17, 40, 3, 90, 60, 33], [1, 1, 1, 1, 1, 1, 1], 8, [0, 1, 2, 3, 4]),  # no row for the sixth
+             ([5, -1, 128, 3, 90, 60, 33], [1, 1, 1, 0, 0, 1, 0], 8, [0, 5]),     # one is no request, one is full
+             ([5, 17, 40, 3, 90, 60, 33], [0] * 7, 8, [])]
+    graph = None
+    if recorded:
+        context.fill_(1)
+        query[:room].fill_(1)
+        height.fill_(8)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+            side.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                made = step()
+        torch.cuda.synchronize()
+    for lens, new, pages, served in cases * 2:
+        context.copy_(torch.tensor(lens)), query.copy_(torch.tensor(new)), height.fill_(pages), table.copy_(table0)
+        torch.cuda.synchronize()
+        if recorded:
+            graph.replay()
+            torch.cuda.synchronize()
+        else:
+            made = step()
+        plan, q, out4, out = made
+        assert [i for i in range(r) if plan.served[i] and new[i]] == served
+        each = torch.zeros(r, hq, d, dtype=BF, device=DEV)  # a row a request, by the list
+        for row, i in enumerate(served):
+            assert int(plan.seq_lens[i]) == lens[i] + 1 and int(plan.positions[row]) == lens[i]
+            each[i] = q[row]
+        want = fq.split_k_paged_decode_dense(each, kc, vc, table, plan.seq_lens)
+        want4 = fq.split_k_paged_decode(each, packed, table, plan.seq_lens, ck, cv, rot, hkv, d, block)
+        assert torch.equal(out[:len(served)], want[served]) and torch.equal(out4[:len(served)], want4[served])
+    if graph is not None:
+        graph.reset()
