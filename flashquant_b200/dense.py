@@ -377,8 +377,10 @@ def split_k_paged_decode_dense(q, key_cache, value_cache, block_table, seq_lens,
     head_dim 64, 96, 128 or 256; block_size a multiple of 16; rows of the caches start at multiples of 16
     bytes; up to 2048 sequences.  Keys and values of visible tokens must be finite; what other rows hold does
     not matter.  A page id out of range is skipped, a length beyond the block table cut, both noted in word 0
-    of the workspace (``workspace_status``).  ``workspace``: ``dense_workspace`` bytes, the first 32 KiB zero
-    before the first use; one per concurrent call.
+    of the workspace (``workspace_status``), the stream's ``dense_workspace`` unless one is given.  ``workspace``: as many
+    uint8, the first 32 KiB zero before the first use; one per concurrent call.  A call that is recorded in a graph
+    without one has memory of its own, whose status nobody sees: replays that are to be looked at are given one (one per
+    graph where graphs run side by side).
     """
     if workspace is None:
         r = _host().dense_decode(q, key_cache, value_cache, block_table, seq_lens, sm_scale, window, out, return_lse)

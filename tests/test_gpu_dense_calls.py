@@ -171,3 +171,26 @@ def test_a_step_that_not_every_request_takes_part_in(consts, recorded):
         assert torch.equal(out[:len(served)], want[served]) and torch.equal(out4[:len(served)], want4[served])
     if graph is not None:
         graph.reset()
+
+
+def test_status_of_replays():
+    """A recorded call leaves its status in the workspace it was given; the stream's own says nothing of it."""
+    b = Batch([40, 700], 32, 8, 128, BF)
+    want = b.call()
+    stream = fq.dense_workspace(DEV, 2, 32, 8, 128)
+    ws = torch.zeros_like(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        given, own = b.call(workspace=ws), b.call()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(given, want) and torch.equal(own, want) and K.workspace_status(ws) == 0
+    page = int(b.table[0, 1])
+    b.table[0, 1] = b.k.shape[0]
+    graph.replay()
+    assert K.workspace_status(ws, reset=True) == N.FQ_DEV_BAD_BLOCK_INDEX and K.workspace_status(stream) == 0
+    assert torch.equal(given, own) and torch.equal(given[1], want[1])
+    b.table[0, 1] = page
+    graph.replay()
+    assert K.workspace_status(ws) == 0 and torch.equal(given, want) and not ws[:32768].any()
+    graph.reset()
