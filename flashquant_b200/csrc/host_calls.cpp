@@ -96,8 +96,12 @@ T* data(const Tensor& t) { return static_cast<T*>(t.data_ptr()); }
 // Workspaces: one per (device, stream, use), zero at first use, grown on demand.  Calls on
 // different streams may overlap on the GPU and must not share counters or partial rows.  None is given
 // back: a call recorded in a CUDA graph keeps the address, so a workspace that was outgrown stays too
-// (each is at least twice its predecessor, all of them together less than twice the last).
+// (each is at least twice its predecessor, all of them together less than twice the last).  Those of the
+// attention over 16-bit pages are as large as they have to be: 30 to 130 MB whatever the batch, by the heads, of which only
+// the first 32 KiB have to be zero.
 // ------------------------------------------------------------------------------------
+enum { kDecode = 0, kAttention = 1, kDense = 2 };  // uses
+constexpr int64_t kDenseHead = 32768;
 struct Workspace {
   std::vector<Tensor> kept;  // the last one is in use
   std::mutex calls;          // held while a call that uses it is enqueued
@@ -121,8 +125,9 @@ Tensor workspace(int dev, int use, size_t bytes, std::mutex** calls = nullptr) {
     }
   }
   // (not under the lock: an allocation may run Python code, which may pass the interpreter on)
-  Tensor t = at::zeros({int64_t(std::max(bytes, 2 * have))},
-                       at::TensorOptions().device(at::kCUDA, dev).dtype(at::kByte));
+  const int64_t size = int64_t(use == kDense ? bytes : std::max(bytes, 2 * have));
+  Tensor t = at::empty({size}, at::TensorOptions().device(at::kCUDA, dev).dtype(at::kByte));
+  t.narrow(0, 0, use == kDense ? std::min(size, kDenseHead) : size).zero_();
   std::lock_guard<std::mutex> lock(g_ws_mutex);
   auto& kept = workspaces()[key].kept;
   if (kept.empty() || size_t(kept.back().numel()) < size_t(t.numel())) kept.push_back(t);
@@ -141,7 +146,6 @@ int native(std::mutex* calls, F call) {
   if (calls) lock = std::unique_lock<std::mutex>(*calls);
   return call();
 }
-enum { kDecode = 0, kAttention = 1, kDense = 2 };
 
 // Bytes for one call: what a call writes and reads back within itself is not shared with another one.
 Tensor call_bytes(int dev, size_t bytes, bool zero) {
@@ -719,7 +723,7 @@ PyObject* dense_decode(PyObject*, Args a, Py_ssize_t n) {
   if (!decode_out(a[7], *q, dev, out)) return none();
   if (a[8] == Py_True) lse = at::empty({seqs, hq}, q->options().dtype(at::kFloat));
   const int hkv = int(kc->size(2));
-  const size_t need = std::max<size_t>(fq_dense_paged_decode_workspace_bytes(int(seqs), int(hq), hkv, int(d)), 32768);
+  const size_t need = std::max<size_t>(fq_dense_paged_decode_workspace_bytes(int(seqs), int(hq), hkv, int(d)), kDenseHead);
   // A call that is being recorded has a workspace of its own: two graphs that hold the stream's would share its
   // counters when they run side by side.
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
@@ -729,7 +733,7 @@ PyObject* dense_decode(PyObject*, Args a, Py_ssize_t n) {
     ws = workspace(dev, kDense, need);
   } else {
     ws = call_bytes(dev, need, false);
-    ws.narrow(0, 0, 32768).zero_();
+    ws.narrow(0, 0, kDenseHead).zero_();
   }
   const int rc = native(nullptr, [&] {  // (the entry has a lock of its own, for callers of every path)
     return fq_dense_paged_decode(

@@ -36,7 +36,9 @@ class _ConvertingCalls:
         kept = self._kept.setdefault((index, torch.cuda.current_stream(index).cuda_stream, use), [])
         have = kept[-1].numel() if kept else 1 << 19
         if not kept or have < need:
-            kept.append(torch.zeros(max(need, 2 * have), dtype=torch.uint8, device=f"cuda:{index}"))
+            size = need if use == _DENSE else max(need, 2 * have)  # (as the extension module does)
+            kept.append(torch.empty(size, dtype=torch.uint8, device=f"cuda:{index}"))
+            kept[-1][:32768 if use == _DENSE else size].zero_()
         return kept[-1]
 
     def workspaces(self, index, use):

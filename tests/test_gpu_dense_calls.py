@@ -194,3 +194,20 @@ def test_status_of_replays():
     graph.replay()
     assert K.workspace_status(ws) == 0 and torch.equal(given, want) and not ws[:32768].any()
     graph.reset()
+
+
+@pytest.mark.parametrize("converted", [False, True])
+def test_workspaces_are_as_large_as_they_have_to_be(monkeypatch, converted):
+    """Heads of another kind take a workspace of their own size, not twice the one before."""
+    if converted:
+        monkeypatch.setattr(K, "_host_module", K._ConvertingCalls())
+    need = lambda *heads: N.load().fq_dense_paged_decode_workspace_bytes(1, *heads)
+    small, large = sorted([(16, 1, 256), (16, 1, 64)], key=lambda h: need(*h))
+    with torch.cuda.stream(torch.cuda.Stream()):
+        for heads, size in ((small, need(*small)), (large, need(*large)), (small, need(*large))):  # (the larger one stays)
+            b = Batch([50, 3000], *heads, HF)
+            b.check(b.call())
+            assert fq.dense_workspace(DEV, 2, *heads).numel() == size
+        ws = fq.dense_workspace(DEV, 2, *large)
+        assert ws.numel() == need(*large) and not ws[:32768].any()
+        torch.cuda.current_stream().synchronize()
