@@ -261,10 +261,11 @@ static int launch_rotary(const RotaryArgs& p, bool half_layout, cudaStream_t str
   const auto kernel = wide ? (half_layout ? rotary_kernel<T, N, true> : rotary_kernel<T, N, false>)
                            : (half_layout ? rotary_kernel<T, 1, true> : rotary_kernel<T, 1, false>);
   const auto smem = [&](int batch) { return 2 * size_t(batch) * (p.rotary_dim / 2) * sizeof(float2); };
-  // A few tokens are spread over more CTAs.  (590 tokens of 40 heads: 4.3, 4.1, 5.3 us with 1, 2, 4 at a time, 148: 3.1,
-  // 3.8, 5.2, 8192: 35.1, 32.2, 32.7, 16384: 66.2, 60.6, 58.4.)
-  int batch = p.tokens <= 592 ? 1 : 2;
-  int64_t ctas = (p.tokens + batch - 1) / batch;
+  // One token at a time as long as each has CTAs of its own that are all resident (bf16, 1 and 2 at a time: 40 heads of 128, 888
+  // resident, 700 tokens 5.7, 6.3 us, 800: 6.2, 6.5, 1000: 7.3, 7.2; 72 heads, 444: 420 tokens 6.1, 6.3, 450: 6.9, 6.6, 592: 8.0,
+  // 7.3; 40 heads with the append, 740: 740 tokens 6.6, 6.7, 800: 7.5, 6.9; 32 of 64, 2368: 1184 tokens 5.1, 5.6, 2300: 7.2, 6.9).
+  int batch = 1;
+  int64_t ctas = p.tokens;
   if (ctas > 64) {  // no more CTAs than are resident together
     int device = 0, sms = 0, fit = 0;
     cudaError_t e = cudaGetDevice(&device);
@@ -272,7 +273,8 @@ static int launch_rotary(const RotaryArgs& p, bool half_layout, cudaStream_t str
     if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, warps * 32, smem(kRotTokens));
     if (e != cudaSuccess) return fail(FQ_ERR_CUDA, "rotary: %s", cudaGetErrorString(e));
     const int64_t most = std::max(1, sms * fit / groups);
-    if (p.tokens > 1184) {
+    if (p.tokens > most) batch = 2;
+    if (batch == 2 && p.tokens > 1184) {
       // what leaves the last round of the CTAs fullest, a token less at a time counted as 2 % more work (8192 tokens:
       // 31.7 us with 4, 30.6 with 3; of heads of 64 19.6 and 18.4)
       int64_t least = INT64_MAX;

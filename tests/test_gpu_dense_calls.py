@@ -211,3 +211,17 @@ def test_workspaces_are_as_large_as_they_have_to_be(monkeypatch, converted):
         ws = fq.dense_workspace(DEV, 2, *large)
         assert ws.numel() == need(*large) and not ws[:32768].any()
         torch.cuda.current_stream().synchronize()
+
+
+@pytest.mark.parametrize("hq, hkv, d", [(32, 8, 128), (64, 8, 128), (8, 1, 64), (128, 8, 128)])
+@pytest.mark.parametrize("n", [65, 296, 444, 445, 593, 888, 889, 1185])
+def test_rotary_around_the_bounds_of_its_rule(hq, hkv, d, n):
+    """However many tokens are taken at a time: the bits of a few tokens alone."""
+    x = torch.randn(n, hq + hkv, d, generator=torch.Generator(device=DEV).manual_seed(n), device=DEV).to(BF)
+    q, k = torch.split(x, (hq, hkv), 1)
+    freq, _ = fq.rotary_frequencies(d, device=DEV)
+    pos = torch.randint(0, 1 << 17, (n,), device=DEV)
+    got = fq.rotary_embed(q, k, pos, freq)
+    for i in range(0, n, 64):
+        part = fq.rotary_embed(q[i:i + 64], k[i:i + 64], pos[i:i + 64], freq)
+        assert all(torch.equal(g[i:i + 64], w) for g, w in zip(got, part))
