@@ -15,12 +15,12 @@
 // and cost nothing.
 //
 // What is left in pieces is joined by a second kernel, launched with the first (programmatic dependent launch).
-// Joined in the first, by the last warp to arrive behind fences and a counter, 1 x 900 tokens took 20 us instead of 9,
+// Joined in the first, by the last warp to arrive behind fences and a counter, 1 x 900 tokens took 20 us instead of 10,
 // and one warp had to read all pieces of a long sequence.
 //
-// Measured (us the call, bytes of the keys and values a second): 32 x 4096, 32 / 8 heads of 128: 93, 5.8 TB/s; ragged
-// 8 x 131072, 64 / 8: 430, 6.8; 48 windows of 1000, 16 / 16 heads of 64: 41, 4.8; 64 x 2000, 16 / 8 of 256: 168, 6.3; 1 x 900:
-// 9 us, of which the first tile is computed at 5 and the join takes 2.
+// Measured (us the call, bytes of the keys and values a second): 32 x 4096, 32 / 8 heads of 128: 94, 5.7 TB/s; ragged
+// 8 x 131072, 64 / 8: 433 - 445, 6.6; 48 windows of 1000, 16 / 16 heads of 64: 43, 4.6; 64 x 2000, 16 / 8 of 256: 166, 6.3; 1 x
+// 900: 10.3 us, of which the first tile is computed at 5 and the join takes 3.
 #include <algorithm>
 #include <mutex>
 
@@ -63,7 +63,7 @@ struct DenseArgs {
 };
 
 // Warps of a CTA, one CTA per SM: as many as the registers leave (a row of the accumulators is D floats).  head_dim 64,
-// 48 x 1000 tokens: 54 us with 8, 39 with 16.
+// 48 x 1000 tokens: 45 us with 8, 41 with 16.
 __host__ __device__ constexpr int dense_warps(int d) { return d == 64 ? 16 : (d > 128 ? 4 : 8); }
 
 template <int D, bool R16>
@@ -77,7 +77,7 @@ struct DenseShape {
   static constexpr int kDescribed = kWarps * 32 * 16;  // 32 tiles of a warp
   // An A operand is four registers in a row: with up to 8 query heads half of them are zeros, 64 registers in all at
   // head_dim 256, which spills (64 x 2000 tokens, 16 / 8 heads: 198 - 219 us).  There the queries stand in shared
-  // memory, and a chunk of zeros for the other rows (168 us).
+  // memory, and a chunk of zeros for the other rows (166 us).
   static constexpr bool kQueries = D == 256 && !R16;
   static constexpr int kQuery = 8 * kRow;
   static constexpr int kZeros = kWarps * kRing + kDescribed + kWarps * kQuery;
@@ -543,8 +543,8 @@ __global__ void __launch_bounds__(kJoinThreads, 8) dense_join_kernel(const Dense
   const int row = column * 4 / p.join_wide;
   const int dim = wide * p.join_wide + column * 4 - row * p.join_wide;
   // Nothing that another kernel has written is read before this wait, the lengths neither: the first kernel has waited for
-  // what came before it, but what a kernel sees is promised behind a wait of its own only.  No CTA leaves before it: this
-  // kernel must not end before the first one has.
+  // what came before it, but what a kernel sees is promised behind a wait of its own only (1 x 900 tokens: 9.5 us with the
+  // lengths read before it).  No CTA leaves before it: this kernel must not end before the first one has.
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int s0 = p.bounds[seq], tiles = (p.bounds[seq + 1] - s0) / unit_groups, total = p.bounds[p.seqs];
@@ -676,7 +676,7 @@ struct DenseGeometry {
   bool r16;
 };
 // Up to 8 query heads to a unit, 16 where a KV head has more: its keys are then read half as often (64 x 4000 tokens, 20 / 2
-// heads: 70 us with units of 8, 55 with 16; 32 / 2: 71, 55).
+// heads: 71 us with units of 8, 56 with 16; 32 / 2: 72, 57).
 static DenseGeometry dense_geometry(int hq, int hkv, int d) {
   DenseGeometry x;
   x.group = hq / hkv;
@@ -734,9 +734,9 @@ static int launch_dependent(void (*kernel)(DenseArgs), const DenseArgs& p, dim3 
 }
 
 // As few heads to a CTA of the join as leave it with eight CTAs on an SM, all resident at once.  Where that leaves room, the
-// pieces of a unit are split over a cluster, 64 or fewer to a CTA (1 x 131072 tokens, 8 query heads on one KV head: 55 us the
-// call without, 25 with), and the dimensions of a head where it still has more than 24 (1 x 900: 13.7 us with whole
-// heads, 10.1 with 32 dimensions; 1 x 32768: 35.9 with the dimensions split first, 32.4 like this).
+// pieces of a unit are split over a cluster, 64 or fewer to a CTA (1 x 131072 tokens, 8 query heads on one KV head: 47 us the
+// call without, 27 with), and the dimensions of a head where it still has more than 24 (1 x 900: 13.9 us with whole
+// heads, 10.3 with 32 dimensions; 1 x 32768: 33.6 whichever is split first).
 template <typename T, int D>
 static int launch_join(DenseArgs p, cudaStream_t stream) {
   const int64_t units = int64_t(p.seqs) * p.hkv * p.chunks, most = 8 * kDenseMaxCtas;

@@ -42,8 +42,8 @@ FQ_HD DenseSpan dense_span(int len, int64_t room, int window) {
 }
 
 // Tiles of a share from which on there is a tail.  Queries, pieces and their join cost more than the balance gives below:
-// 32 x 4096 tokens (a share of 55) 92 us without, 92 - 100 with one; 64 x 2000, head_dim 256 (108) 198, 201 - 219; ragged
-// 8 x 131072 (300) 445 and, after other data, 500 without, 428 and 475 with one.
+// 32 x 4096 tokens (a share of 55) 94 us without, 94 with one; 64 x 2000, head_dim 256 (108) 166, 170; ragged 8 x 131072
+// (300) 452 without, 433 with one.
 constexpr int kDenseShare = 192;
 constexpr int kDenseMain = 14;    // entries of sixteen that are not in the tail
 constexpr int kDenseTaken = 4;    // runs taken per share, at most

@@ -13,8 +13,9 @@
 // (With rows of all three tensors dealt to the threads of a CTA the same work took 240 instructions to a place and
 // three times as long.)
 //
-// Measured, 32 / 8 heads of 128, bf16: 32 tokens 2.9 us, with the append 3.2; 8192 tokens 30.6 us, 36.4 with it: 5.5 TB/s
-// read and written, 84 % of a copy (16384 tokens: 91 %); the loads that 24 warps of an SM have under way bound it.
+// Measured, 32 / 8 heads of 128, bf16: 32 tokens 3.1 us, with the append 3.4; 8192 tokens 31.2 us, 37.5 with it: 5.4 TB/s
+// read and written, 82 % of a copy (16384 tokens: 89 %); the loads that 30 warps of an SM have under way bound it.  Rows that
+// are not whole vectors of 16 bytes go value by value: 8192 tokens of 96 values, 48 of them rotated 28.1 us, 24 of them 67.6.
 #include <algorithm>
 
 #include "fq_common.cuh"

@@ -7,8 +7,8 @@
 // written before all CTAs have read it: then they are one cluster, which has a barrier; else as many as there is work
 // for.
 //
-// Measured: 256 requests of a token each 5.0 us, 64 prompts of 39 000 tokens 5.5, 1024 requests with 128 000 pages
-// released 4.4; of these the launch takes 2, the lengths and the scan 2.
+// Measured: 256 requests of a token each 5.5 us, 64 prompts of 39 000 tokens 5.9, 1024 requests with 128 000 pages
+// released 4.6; of these the launch takes 2, the lengths and the scan 2.
 #include <algorithm>
 
 #include "fq_common.cuh"
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(kPlanThreads) release_pages_kernel(const Relea
   if (cta == 0 && tid == 0) *p.count_out = int32_t(height + total);
 }
 
-// (64 prompts, 39 000 tokens: 10.2 us by a cluster of eight CTAs, 5.5 by one to 1024; 128 000 pages released: 15.3, 4.4)
+// (64 prompts, 39 000 tokens: 10.1 us by a cluster of eight CTAs, 5.9 by one to 1024; 128 000 pages released: 14.9, 4.6)
 constexpr int kPlanCluster = 8, kPlanMaxCtas = 148;
 // `work`: pages or tokens
 template <typename Args>
