@@ -1,5 +1,6 @@
 // Library-wide pieces of the C ABI: version and the per-thread error text.
 #include <atomic>
+#include <mutex>
 
 #include "fq_common.cuh"
 
@@ -7,6 +8,11 @@ namespace fq {
 char* last_error_buffer() {
   static thread_local char buf[512] = {0};
   return buf;
+}
+std::mutex& workspace_calls(const void* workspace) {
+  static std::mutex locks[64];
+  const uintptr_t at = reinterpret_cast<uintptr_t>(workspace);
+  return locks[(at >> 9 ^ at >> 21) % 64];
 }
 static std::atomic<uint64_t> g_launches{0};
 void count_launch(uint64_t n) { g_launches.fetch_add(n, std::memory_order_relaxed); }

@@ -22,7 +22,6 @@
 // 8 x 131072, 64 / 8: 433 - 445, 6.6; 48 windows of 1000, 16 / 16 heads of 64: 43, 4.6; 64 x 2000, 16 / 8 of 256: 166, 6.3; 1 x
 // 900: 10.3 us, of which the first tile is computed at 5 and the join takes 3.
 #include <algorithm>
-#include <mutex>
 
 #include <cooperative_groups.h>
 
@@ -798,14 +797,6 @@ static int launch_dense(const DenseArgs& p, int d, bool r16, int ctas, cudaStrea
   }
 }
 
-// Held while the two kernels of a call are enqueued: threads that share a stream share its workspace, and the first kernel
-// of one call must not come between those of another.  (Some workspaces share a lock.)
-static std::mutex& dense_calls(const void* workspace) {
-  static std::mutex locks[64];
-  const uintptr_t at = reinterpret_cast<uintptr_t>(workspace);
-  return locks[(at >> 9 ^ at >> 21) % 64];
-}
-
 }  // namespace fq
 
 using namespace fq;
@@ -881,7 +872,7 @@ extern "C" int fq_dense_paged_decode(
   const int64_t runs = (most + kDenseShortest - 1) / kDenseShortest;
   const int ctas = int(std::max<int64_t>(1, std::min<int64_t>(sms, (runs + teams - 1) / teams)));
   p.fixed = ctas * teams;
-  std::lock_guard<std::mutex> enqueued(dense_calls(workspace));
+  std::lock_guard<std::mutex> enqueued(workspace_calls(workspace));
   return dtype == FQ_F16 ? launch_dense<__half>(p, head_dim, x.r16, ctas, stream)
                          : launch_dense<__nv_bfloat16>(p, head_dim, x.r16, ctas, stream);
 }

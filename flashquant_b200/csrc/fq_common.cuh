@@ -10,6 +10,7 @@
 
 #include <cstdarg>
 #include <cstdio>
+#include <mutex>
 
 #include "../../include/flashquant_b200.h"
 
@@ -31,6 +32,11 @@ inline int fail(int code, const char* fmt, ...) {
 void count_launch(uint64_t n = 1);  // library-wide counter of kernel launches (capi.cu)
 uint64_t settings_epoch();  // changes whenever a process-wide setter is called (capi.cu)
 void settings_changed();
+
+// Held while the launches of a call that has a workspace are enqueued: threads that share a stream share its
+// workspace, and no launch of one call may come between those of another.  In the C entries, so that it holds for callers of
+// every path.  (Some workspaces share a lock.)
+std::mutex& workspace_calls(const void* workspace);
 
 inline int check_launch(const char* what) {
   cudaError_t e = cudaGetLastError();

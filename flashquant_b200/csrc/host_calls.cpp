@@ -102,26 +102,21 @@ T* data(const Tensor& t) { return static_cast<T*>(t.data_ptr()); }
 // ------------------------------------------------------------------------------------
 enum { kDecode = 0, kAttention = 1, kDense = 2 };  // uses
 constexpr int64_t kDenseHead = 32768;
-struct Workspace {
-  std::vector<Tensor> kept;  // the last one is in use
-  std::mutex calls;          // held while a call that uses it is enqueued
-};
+using Kept = std::vector<Tensor>;  // the last one is in use
 std::mutex g_ws_mutex;
-std::map<std::tuple<int, const void*, int>, Workspace>& workspaces() {
-  static auto* m = new std::map<std::tuple<int, const void*, int>, Workspace>();
+std::map<std::tuple<int, const void*, int>, Kept>& workspaces() {
+  static auto* m = new std::map<std::tuple<int, const void*, int>, Kept>();
   return *m;  // never destroyed: the CUDA context may be gone at exit
 }
-// `calls`: receives the lock of the workspace's calls
-Tensor workspace(int dev, int use, size_t bytes, std::mutex** calls = nullptr) {
+Tensor workspace(int dev, int use, size_t bytes) {
   const auto key = std::make_tuple(dev, static_cast<const void*>(stream_of(dev)), use);
   size_t have = size_t(1) << 19;
   {
     std::lock_guard<std::mutex> lock(g_ws_mutex);
-    Workspace& w = workspaces()[key];
-    if (calls) *calls = &w.calls;
-    if (!w.kept.empty()) {
-      have = size_t(w.kept.back().numel());
-      if (have >= bytes) return w.kept.back();
+    const Kept& kept = workspaces()[key];
+    if (!kept.empty()) {
+      have = size_t(kept.back().numel());
+      if (have >= bytes) return kept.back();
     }
   }
   // (not under the lock: an allocation may run Python code, which may pass the interpreter on)
@@ -129,21 +124,19 @@ Tensor workspace(int dev, int use, size_t bytes, std::mutex** calls = nullptr) {
   Tensor t = at::empty({size}, at::TensorOptions().device(at::kCUDA, dev).dtype(at::kByte));
   t.narrow(0, 0, use == kDense ? std::min(size, kDenseHead) : size).zero_();
   std::lock_guard<std::mutex> lock(g_ws_mutex);
-  auto& kept = workspaces()[key].kept;
+  Kept& kept = workspaces()[key];
   if (kept.empty() || size_t(kept.back().numel()) < size_t(t.numel())) kept.push_back(t);
   return kept.back();
 }
-// The native call without the interpreter lock (a full launch queue makes it wait), and alone among the
-// calls that use the same workspace: it may be several launches.
+// The native call without the interpreter lock: a full launch queue makes it wait, and so do the calls of other threads that
+// use the same workspace.
 struct WithoutInterpreter {
   PyThreadState* state = PyEval_SaveThread();
   ~WithoutInterpreter() { PyEval_RestoreThread(state); }
 };
 template <typename F>
-int native(std::mutex* calls, F call) {
+int native(F call) {
   WithoutInterpreter released;
-  std::unique_lock<std::mutex> lock;
-  if (calls) lock = std::unique_lock<std::mutex>(*calls);
   return call();
 }
 
@@ -163,9 +156,9 @@ PyObject* py_workspaces(PyObject*, Args a, Py_ssize_t n) {
   std::vector<Tensor> found;
   {
     std::lock_guard<std::mutex> lock(g_ws_mutex);
-    for (const auto& [key, w] : workspaces())
+    for (const auto& [key, kept] : workspaces())
       if (std::get<0>(key) == dev && std::get<2>(key) == use)
-        found.insert(found.end(), w.kept.begin(), w.kept.end());
+        found.insert(found.end(), kept.begin(), kept.end());
   }
   PyObject* list = PyList_New(0);
   for (const Tensor& t : found) {
@@ -230,7 +223,7 @@ PyObject* compress_append(PyObject*, Args a, Py_ssize_t n) {
   const Tensor *rot = f32(a[4], dev), *bk = f32(a[5], dev);
   const Tensor* bv = a[6] == Py_None ? bk : f32(a[6], dev);
   if (!rot || !bk || !bv || !append_args(a[0], a[1], a[2], a[3], dev, p)) return none();
-  return done(native(nullptr, [&] {
+  return done(native([&] {
     return fq_tq4_compress_append(
       p.key->data_ptr(), p.value->data_ptr(), fq_dtype(p.dt), p.n, p.h, p.d, p.stride, data(*rot),
       data(*bk), int(bk->numel()), data(*bv), int(bv->numel()), data<uint8_t>(*p.cache),
@@ -253,7 +246,7 @@ PyObject* compress_append_qjl(PyObject*, Args a, Py_ssize_t n) {
       plane->size(0) * plane->size(1) != p.num_slots || s->dim() != 2 || s->size(0) != p.d ||
       s->size(1) != p.d || ck->numel() != bk->numel() + 1)
     return none();
-  return done(native(nullptr, [&] {
+  return done(native([&] {
     return fq_tq4_compress_append_qjl(
       p.key->data_ptr(), p.value->data_ptr(), fq_dtype(p.dt), p.n, p.h, p.d, p.stride, data(*rot),
       data(*bk), int(bk->numel()), data(*ck), data(*bv), int(bv->numel()), data(*s),
@@ -318,10 +311,9 @@ PyObject* paged_decode(PyObject*, Args a, Py_ssize_t n) {
   Tensor out;
   if (!decode_args(a, a[10], a[12], dev, 3, p) || !decode_out(a[11], *p.q, dev, out)) return none();
   const int seqs = int(p.q->size(0));
-  std::mutex* calls;
   Tensor ws = workspace(dev, kDecode,
-                        fq_paged_decode_workspace_bytes(seqs, p.hq, p.hkv, p.d, p.splits), &calls);
-  return done(native(calls, [&] {
+                        fq_paged_decode_workspace_bytes(seqs, p.hq, p.hkv, p.d, p.splits));
+  return done(native([&] {
     return fq_split_k_paged_decode(
                   p.q->data_ptr(), fq_dtype(p.dt), data<uint8_t>(*p.cache), data<int32_t>(*p.table),
                   p.table->stride(0), data<int32_t>(*p.lens), data(*p.ck), int(p.ck->numel()),
@@ -347,10 +339,9 @@ PyObject* paged_decode_qjl(PyObject*, Args a, Py_ssize_t n) {
       s->size(1) != p.d)
     return none();
   const int seqs = int(p.q->size(0));
-  std::mutex* calls;
   Tensor ws = workspace(dev, kDecode,
-                        fq_paged_decode_workspace_bytes(seqs, p.hq, p.hkv, p.d, p.splits), &calls);
-  return done(native(calls, [&] {
+                        fq_paged_decode_workspace_bytes(seqs, p.hq, p.hkv, p.d, p.splits));
+  return done(native([&] {
     return fq_split_k_paged_decode_qjl(
                   p.q->data_ptr(), fq_dtype(p.dt), data<uint8_t>(*p.cache), data<uint8_t>(*plane),
                   data<int32_t>(*p.table), p.table->stride(0), data<int32_t>(*p.lens), data(*p.ck),
@@ -371,17 +362,15 @@ PyObject* paged_decode_multi(PyObject*, Args a, Py_ssize_t n) {
   if (seqs == 0 || n_q == 0) return none();
   Tensor out = at::empty(p.q->sizes(), p.q->options());
   const int max_blocks = int(p.table->size(1));
-  std::mutex* calls;
   Tensor ws = workspace(dev, kDecode,
                         std::max(fq_split_k_paged_decode_multi_workspace_bytes(
                                      seqs, n_q, p.hq, p.hkv, p.d, p.splits),
                                  fq_paged_decode_workspace_bytes(seqs * n_q, p.hq, p.hkv, p.d,
-                                                                 p.splits)),
-                        &calls);
+                                                                 p.splits)));
   Tensor scratch = call_bytes(
       dev, std::max<size_t>(fq_split_k_paged_decode_multi_scratch_bytes(seqs, n_q, max_blocks), 16),
       false);
-  return done(native(calls, [&] {
+  return done(native([&] {
     return fq_split_k_paged_decode_multi(
                   p.q->data_ptr(), fq_dtype(p.dt), data<uint8_t>(*p.cache), data<int32_t>(*p.table),
                   p.table->stride(0), max_blocks, data<int32_t>(*p.lens), data(*p.ck),
@@ -408,7 +397,7 @@ PyObject* paged_prefill(PyObject*, Args a, Py_ssize_t n) {
     return none();
   const int total = int(p.q->size(0));
   Tensor ws = call_bytes(dev, fq_paged_tq4_prefill_workspace_bytes(total, p.hq, p.d), true);
-  return done(native(nullptr, [&] {
+  return done(native([&] {
     return fq_paged_tq4_prefill(
                   p.q->data_ptr(), fq_dtype(p.dt), data<uint8_t>(*p.cache), data<int32_t>(*p.table),
                   p.table->stride(0), data<int32_t>(*p.lens), data<int32_t>(*cu), data(*p.ck),
@@ -433,7 +422,7 @@ PyObject* compress(PyObject*, Args a, Py_ssize_t n) {
   const int64_t nt = x->size(0), h = x->size(1), d = x->size(2);
   Tensor packed = at::empty({nt, h, d / 2}, x->options().dtype(at::kByte));
   Tensor norms = at::empty({nt, h, 1}, x->options().dtype(at::kFloat));
-  const int rc = native(nullptr, [&] {
+  const int rc = native([&] {
     return fq_tq4_compress(x->data_ptr(), fq_dtype(dtype_code(*x)), data(*even), data(*odd),
                                  data(*bnd), int(bnd->numel()), data<uint8_t>(packed), data(norms),
                                  nt * h, int(d), stream_of(dev));
@@ -487,9 +476,8 @@ PyObject* attention(PyObject*, Args a, Py_ssize_t n) {
   const int64_t cap = view_capacity(*kv[0], *kv[1]);
   if (cap == 0 || view_capacity(*kv[2], *kv[3]) != cap) return none();
   Tensor out = at::empty(q->sizes(), q->options());
-  std::mutex* calls;
-  Tensor ws = workspace(dev, kAttention, fq_fused_tq_attention_workspace_bytes(b, hq, nq, d), &calls);
-  return done(native(calls, [&] {
+  Tensor ws = workspace(dev, kAttention, fq_fused_tq_attention_workspace_bytes(b, hq, nq, d));
+  return done(native([&] {
     return fq_fused_tq_attention_kv(
                   q->data_ptr(), fq_dtype(dtype_code(*q)), data<uint8_t>(*kv[0]), data(*kv[1]),
                   data<uint8_t>(*kv[2]), data(*kv[3]), data(*ck), int(ck->numel()), data(*cv),
@@ -546,7 +534,7 @@ PyObject* cache_update(PyObject*, Args a, Py_ssize_t n) {
   } else if (a[10] != Py_None) {
     return none();
   }
-  return done(native(nullptr, [&] {
+  return done(native([&] {
     return fq_cache_update(
       key->data_ptr(), val->data_ptr(), fq_dtype(dtype_code(*key)), data(*tk[0]), data(*tk[1]),
       data(*tk[4]), data(*tv[0]), data(*tv[1]), data(*tv[4]), data(*tk[2]), int(tk[2]->numel()),
@@ -656,7 +644,7 @@ PyObject* rotary_embed(PyObject*, Args a, Py_ssize_t n) {
   }
   const int64_t strides[8] = {q->stride(0), q->stride(1), k ? k->stride(0) : 0, k ? k->stride(1) : 0,
                               q_out.stride(0), q_out.stride(1), k ? k_out.stride(0) : 0, k ? k_out.stride(1) : 0};
-  const int rc = native(nullptr, [&] {
+  const int rc = native([&] {
     return fq_rotary_embed(q->data_ptr(), k ? k->data_ptr() : nullptr, fq_dtype(dtype_code(*q)), tokens,
                            int(q->size(1)), k ? int(k->size(1)) : 0, int(d), int(2 * freq->size(0)), strides,
                            pos->data_ptr(), is_long(*pos), data<double>(*freq), fq_rotary_layout(layout),
@@ -690,7 +678,7 @@ PyObject* rotary_append_dense(PyObject*, Args a, Py_ssize_t n) {
   const int64_t strides[14] = {q->stride(0), q->stride(1), key->stride(0), key->stride(1), val->stride(0),
                                val->stride(1), q_out.stride(0), q_out.stride(1), kc->stride(0), kc->stride(1),
                                kc->stride(2), vc->stride(0), vc->stride(1), vc->stride(2)};
-  return done(native(nullptr, [&] {
+  return done(native([&] {
     return fq_rotary_append_dense(
                   q->data_ptr(), key->data_ptr(), val->data_ptr(), fq_dtype(dtype_code(*key)), tokens,
                   int(q->size(1)), int(h), int(d), int(2 * freq->size(0)), strides, pos->data_ptr(), is_long(*pos),
@@ -735,7 +723,7 @@ PyObject* dense_decode(PyObject*, Args a, Py_ssize_t n) {
     ws = call_bytes(dev, need, false);
     ws.narrow(0, 0, kDenseHead).zero_();
   }
-  const int rc = native(nullptr, [&] {  // (the entry has a lock of its own, for callers of every path)
+  const int rc = native([&] {
     return fq_dense_paged_decode(
         q->data_ptr(), fq_dtype(dtype_code(*q)), q->stride(0), q->stride(1), kc->data_ptr(), kc->stride(0),
         kc->stride(1), kc->stride(2), vc->data_ptr(), vc->stride(0), vc->stride(1), vc->stride(2),
@@ -801,7 +789,7 @@ PyObject* plan_paged_step(PyObject*, Args a, Py_ssize_t n) {
   out[3] = piece(room, at::kLong);
   out[4] = piece(r, at::kBool);
   out[5] = p.count_out.defined() ? p.count_out : piece(1, at::kInt);
-  const int rc = native(nullptr, [&] {
+  const int rc = native([&] {
     return fq_plan_paged_step(data<int32_t>(*context), data<int32_t>(*query), int(p.requests), data<int32_t>(*p.table),
                               p.stride, int(p.width), int(p.block_size), data<int32_t>(*p.free), p.free->numel(),
                               data<int32_t>(*p.count), room, data<int32_t>(out[0]), data<int32_t>(out[1]),
@@ -825,7 +813,7 @@ PyObject* release_pages(PyObject*, Args a, Py_ssize_t n) {
       context->size(0) != p.requests)
     return none();
   if (!p.count_out.defined()) p.count_out = at::empty({1}, p.count->options());
-  return done(native(nullptr, [&] {
+  return done(native([&] {
     return fq_release_pages(data<uint8_t>(*finished), data<int32_t>(*context), int(p.requests),
                             data<int32_t>(*p.table), p.stride, int(p.width), int(p.block_size),
                             data<int32_t>(*p.free), p.free->numel(), data<int32_t>(*p.count),

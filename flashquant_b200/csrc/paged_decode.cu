@@ -1935,6 +1935,7 @@ static int decode_call(const void* q, fq_dtype dtype, const uint8_t* kv_cache,
   if (rc != FQ_OK) return rc;
   FQ_REQUIRE(out && aligned(out, 2), FQ_ERR_INVALID_ARGUMENT, "paged decode: out is null");
   if (num_seqs == 0) return FQ_OK;
+  std::lock_guard<std::mutex> enqueued(workspace_calls(workspace));
   const int ctas = device_sm_count();
   if (num_splits == 0) num_splits = auto_splits();
   // an fp32 query (the reference's CPU-sized cases) takes the three-launch form: its rotated
@@ -2026,6 +2027,7 @@ extern "C" int fq_split_k_paged_decode_qjl(
   FQ_REQUIRE(aligned(kq_cache, 16) && aligned(qjl, 16), FQ_ERR_ALIGNMENT,
              "paged decode (two-stage): kq_cache and qjl must be 16-byte aligned");
   if (num_seqs == 0) return FQ_OK;
+  std::lock_guard<std::mutex> enqueued(workspace_calls(workspace));
   const int ctas = device_sm_count();
   if (num_splits == 0) num_splits = auto_splits();
   rc = decode_front(q, dtype, kv_cache, block_table, block_table_stride, seq_lens, centroids_k,
@@ -2052,6 +2054,7 @@ static int partials_common(const void* q, fq_dtype dtype, const uint8_t* kv_cach
   FQ_REQUIRE(partials && aligned(partials, 16), FQ_ERR_ALIGNMENT,
              "partials must be 16-byte aligned");
   if (num_seqs == 0) return FQ_OK;
+  std::lock_guard<std::mutex> enqueued(workspace_calls(workspace));
   const int ctas = device_sm_count();
   if (num_splits == 0) num_splits = auto_splits();
   int rc = decode_front(q, dtype, kv_cache, block_table, block_table_stride, seq_lens,

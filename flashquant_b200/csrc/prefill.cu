@@ -668,6 +668,7 @@ static int attention_common(const void* q, fq_dtype dtype, const uint8_t* k_pack
   const PrefillWorkspace w = prefill_workspace(rows, head_dim, n_q == 1);
   FQ_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= w.total, FQ_ERR_WORKSPACE,
              "fused attention: workspace of %zu bytes needed (256-byte aligned)", w.total);
+  std::lock_guard<std::mutex> enqueued(workspace_calls(workspace));
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   __half* q_rot = reinterpret_cast<__half*>(ws + w.q_rot_off);
   float* o_rot = reinterpret_cast<float*>(ws + w.o_rot_off);

@@ -225,3 +225,29 @@ def test_rotary_around_the_bounds_of_its_rule(hq, hkv, d, n):
     for i in range(0, n, 64):
         part = fq.rotary_embed(q[i:i + 64], k[i:i + 64], pos[i:i + 64], freq)
         assert all(torch.equal(g[i:i + 64], w) for g, w in zip(got, part))
+
+
+@pytest.mark.parametrize("converted", [1, 2])
+def test_compressed_attention_of_converted_arguments_from_two_threads(consts, converted):
+    """Attention over a compressed cache: calls of one thread, or of both, go through the conversion."""
+    bnd, c, rot = (consts[n].contiguous().to(DEV) for n in ("boundaries_128_4", "centroids_128_4", "rotation_128_0"))
+    cases = []
+    for i in range(2):
+        x = torch.randn(2 * 8 * 600, 1, 128, device=DEV, generator=torch.Generator(DEV).manual_seed(i)).half()
+        p, n = fq.tq4_compress(x, rot, bnd)
+        q = torch.randn(2, 32, 1, 128, device=DEV).half()
+        args = (q, p.view(2, 8, 600, 64), n.view(2, 8, 600, 1), p.view(2, 8, 600, 64), n.view(2, 8, 600, 1), c, c, rot)
+        want = fq.fused_tq_attention(*args, sm_scale=1.0)
+        cases.append((args, 1 if i < converted else 1.0, want))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(args, scale, want):
+        outs = [fq.fused_tq_attention(*args, sm_scale=scale) for _ in range(300)]
+        wrong.extend(i for i, o in enumerate(outs) if not torch.equal(o, want))
+    threads = [threading.Thread(target=run, args=case) for case in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
