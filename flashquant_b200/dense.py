@@ -372,7 +372,8 @@ def split_k_paged_decode_dense(q, key_cache, value_cache, block_table, seq_lens,
     ``q`` ``(num_seqs, H_q, D)``, the caches ``(num_blocks, block_size, H_kv, D)`` of its type (fp16 or
     bf16), ``block_table`` ``(num_seqs, width)`` and ``seq_lens`` int32.  ``window``: each sequence sees its
     last ``window`` tokens (0: all).  ``return_lse``: also the fp32 ``(num_seqs, H_q)`` logarithms of the sums
-    of ``exp(sm_scale q k)``.  A sequence without tokens gives zeros (and -inf).
+    of ``exp(sm_scale q k)``.  ``out``: contiguous, at a multiple of 8 bytes.  A sequence without tokens gives zeros
+    (and -inf).
 
     head_dim 64, 96, 128 or 256; block_size a multiple of 16; rows of the caches start at multiples of 16
     bytes; up to 2048 sequences.  Keys and values of visible tokens must be finite; what other rows hold does

@@ -251,3 +251,95 @@ def test_compressed_attention_of_converted_arguments_from_two_threads(consts, co
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("hq, hkv, d", [(2, 2, 256), (16, 1, 256), (8, 8, 128), (4, 1, 64), (6, 2, 96)])
+def test_as_many_sequences_as_a_call_takes(hq, hkv, d):
+    lens = [(7 * i) % 40 for i in range(2047)] + [3000]
+    b = Batch(lens, hq, hkv, d, HF)
+    out, lse = b.call(return_lse=True)
+    b.check(out, lse, only=[0, 1, 2, 40, 777, 2040, 2046, 2047])
+    assert not out.isnan().any() and not out[::40].any()
+    b.sl.zero_()
+    assert not b.call().any()
+
+
+@pytest.mark.parametrize("hq, hkv", [(1024, 1), (1024, 1024), (1000, 8), (17, 17)])
+def test_as_many_heads_as_a_call_takes(hq, hkv):
+    b = Batch([40, 0, 1, 500], hq, hkv, 64, BF)
+    out, lse = b.call(return_lse=True)
+    b.check(out, lse)
+
+
+def test_rotary_offsets_beyond_32_bits():
+    n, hq, d = (1 << 31) // (32 * 128) + 300, 32, 128
+    q = torch.empty(n, hq, d, dtype=BF, device=DEV)
+    q[-400:] = torch.randn(400, hq, d, device=DEV).to(BF)
+    q[:-400] = 0
+    freq, _ = fq.rotary_frequencies(d, device=DEV)
+    pos = torch.arange(n, device=DEV)
+    want, _ = fq.rotary_embed(q[-400:].clone(), None, pos[-400:], freq)
+    got, _ = fq.rotary_embed(q, None, pos, freq)
+    assert torch.equal(got[-400:], want) and not got[:-400].any()
+    fq.rotary_embed(q, None, pos, freq, out=(q, None))
+    assert torch.equal(q[-400:], want) and not q[:-400].any()
+
+
+@pytest.mark.parametrize("requests", [3, 900])
+def test_recorded_plans_in_place(requests):
+    """A plan and a release that update the stack's height in place, replayed with other lengths: large enough for several
+    CTAs, the pages are those that the calls take when they are made one by one."""
+    width, block, blocks, room = 40, 16, 40000, 9000
+    g = torch.Generator().manual_seed(requests)
+    context, query = torch.zeros(requests, **I32), torch.zeros(requests, **I32)
+    done, table = torch.zeros(requests, dtype=torch.bool, device=DEV), torch.zeros(requests, width, **I32)
+    free, height = torch.randperm(blocks, generator=g).int().to(DEV), torch.tensor([blocks], **I32)
+    state = [table, free, height]
+
+    def step():
+        plan = fq.plan_paged_step(context, query, table, free, height, block, room, free_count_out=height)
+        fq.release_pages(done, plan.seq_lens, table, free, height, block, free_count_out=height)
+        return plan
+    graph = torch.cuda.CUDAGraph()
+    step()  # (nothing is asked for)
+    with torch.cuda.graph(graph):
+        made = step()
+    for i in range(8):
+        new = torch.randint(0, 600, (requests,), generator=g).int().to(DEV)
+        query.copy_(torch.where((context + new) <= width * block, new, torch.zeros_like(new)))
+        done.copy_(torch.rand(requests, generator=g) < 0.4)
+        before = [x.clone() for x in state]
+        plan = step()
+        want = [x.clone() for x in (*plan, *state)]
+        for x, y in zip(state, before):
+            x.copy_(y)
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip((*made, *state), want):
+            assert torch.equal(x, y)
+        context.copy_(torch.where(done, torch.zeros_like(context), plan.seq_lens))
+        held = int(((context + block - 1) // block).sum())
+        assert int(height) == blocks - held and plan.served.any()
+        mine = [table[r, :(int(context[r]) + block - 1) // block] for r in range(requests)]
+        assert torch.equal(torch.cat([*mine, free[:int(height)]]).sort().values, torch.arange(blocks, **I32))
+    graph.reset()
+
+
+def test_results_take_part_in_what_follows():
+    """Results that share one allocation: under inference mode, as inputs of a gradient, one of them kept alone."""
+    q, k = (torch.randn(9, h, 128, device=DEV).to(BF) for h in (8, 2))
+    freq, _ = fq.rotary_frequencies(128, device=DEV)
+    pos = torch.arange(9, device=DEV)
+    a, b = fq.rotary_embed(q, k, pos, freq)
+    with torch.inference_mode():
+        c, d = fq.rotary_embed(q, k, pos, freq)
+        assert torch.equal(a, c) and torch.equal(b, d) and c.is_inference()
+        c.add_(1)
+    w = torch.ones(128, device=DEV, dtype=BF, requires_grad=True)
+    (a * w).float().sum().backward()
+    assert torch.isfinite(w.grad).all()
+    kept = b.clone()
+    del a, c, d
+    for _ in range(20):
+        torch.randn(9, 8, 128, device=DEV)
+    assert torch.equal(b, kept) and b.is_contiguous()
